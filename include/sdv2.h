@@ -309,6 +309,64 @@ int sdv2_residual_layernorm(const void* x, const void* y, const void* gate, int6
                             int affine, const void* mul, const void* add, int64_t mod_row_stride, void* out,
                             int batch, int frames, int tokens_per_frame, int dim, float eps, void* stream);
 
+/*
+ * The K/V cache in 8 bits.  Per (row, token, head) vector x of 128 values: an exponent
+ *   e = max(floor(log2(max|x|)) - 6, -126)
+ * and one byte per value, a sign bit above a 7-bit magnitude m = min(rint(|x| / 2^e), 127) (ties to even); the vector
+ * holds sign * m * 2^e, exactly representable in bf16.  |x - held| is at most 2^(e-1), or one step 2^e for a magnitude
+ * above 127.5.  A vector with a value that is infinite, NaN or (after the rope) beyond fp32's range gets e = -128 and
+ * holds NaN.  No reference counterpart (its cache has the model's type, models/wan/causal_stream_inference.py:98-105).
+ *
+ * Caches are byte views [rows, tokens, heads, 128]; strides in bytes, multiples of 16.  Exponents are int8 views
+ * [rows, tokens, heads] (strides in bytes, any alignment; the innermost stride of the view is stride_head).
+ *
+ * sdv2_rope_kv_append_q8: sdv2_rope_kv_append with the slot write in this format.  q_out is that call's q_out bit for
+ *   bit; K is quantised from the fp64 rope result (one rounding), V from its input.  Slot parameters: the host arrays
+ *   start_frame / dst_begin (+ index values) with step_params_dev NULL, or step_params_dev (device int64 [4][rows], as
+ *   for sdv2_rope_kv_append_indirect) with the host arrays NULL.  head_dim must be 128; dtype is that of q, k, v, q_out.
+ * sdv2_kv_read_q8: k_out[b, i], v_out[b, i] = what the cache holds of token begin[b] + i, i < tokens, as bf16 or f32
+ *   (`dtype`; both exact).  begin: host int64[rows], begin[b] + tokens <= cache_tokens.  Cache rows may be broadcast.
+ * sdv2_attn_kvcache_q8: sdv2_attn_kvcache over the values the cache holds.  seq_lens[b] may be 0: that row's output is
+ *   0.  Cache bytes and exponents at and beyond seq_lens[b] may hold anything.  scratch_dev: at least
+ *   sdv2_attn_q8_scratch_bytes() bytes (may be 0: then NULL), 16-byte aligned, no initialisation needed; one call's
+ *   own, calls that may overlap on the GPU need one each.  status_dev as for sdv2_rope_kv_append.
+ */
+int sdv2_rope_kv_append_q8(const sdv2_view* q, const sdv2_view* k, const sdv2_view* v, const sdv2_view* q_out,
+                           const sdv2_view* k_cache, const sdv2_view* v_cache, const sdv2_view* k_exp,
+                           const sdv2_view* v_exp, int rows, int new_tokens, int heads, int head_dim,
+                           int64_t cache_tokens, const double* rope_table_dev, int table_rows, int grid_f, int grid_h,
+                           int grid_w, const int64_t* start_frame, const int64_t* dst_begin,
+                           const int64_t* step_params_dev, int64_t* global_end_dev, int64_t* local_end_dev,
+                           const int64_t* global_end_val, const int64_t* local_end_val, int dtype, int* status_dev,
+                           void* stream);
+int sdv2_kv_read_q8(const sdv2_view* k_cache, const sdv2_view* v_cache, const sdv2_view* k_exp, const sdv2_view* v_exp,
+                    const sdv2_view* k_out, const sdv2_view* v_out, int rows, int tokens, int heads, int head_dim,
+                    int64_t cache_tokens, const int64_t* begin, int dtype, void* stream);
+int sdv2_attn_kvcache_q8(const sdv2_view* q, const sdv2_view* k_cache, const sdv2_view* v_cache, const sdv2_view* k_exp,
+                         const sdv2_view* v_exp, const sdv2_view* out, int rows, int q_tokens, int heads, int head_dim,
+                         int64_t cache_tokens, const int32_t* seq_lens, float softmax_scale, void* scratch_dev,
+                         size_t scratch_bytes, int* status_dev, void* stream);
+size_t sdv2_attn_q8_scratch_bytes(int rows, int q_tokens, int heads, int64_t cache_tokens, const int32_t* seq_lens);
+
+/*
+ * Attention in which query i of row b attends the keys begin[b, i] <= j < end[b, i] and no others: prompt lengths
+ * (begin 0, end the length), block-causal clips (end the end of the query's block), packed clips (begin and end of the
+ * query's own), windows.  Spans are clipped to [0, kv_tokens); a query whose span is empty gets 0.
+ * Covers WanT2VCrossAttention.forward with context_lens (models/wan/wan_base/modules/model.py:161-194) and the masks of
+ * CausalWanSelfAttention.forward without a cache (models/wan/causal_model.py:219-248).
+ *
+ * bf16 in and out, fp32 accumulate, head_dim 128; k / v stride_row may be 0.  begin_dev (NULL: 0) and end_dev: device
+ * int32, element strides per row and per query, 0 allowed (one span for all); read when the kernel runs.
+ * K and V of keys that no query attends may hold anything, NaN included.
+ * scratch_dev, status_dev: as for sdv2_attn_kvcache_q8, with sdv2_attn_spans_scratch_bytes().
+ */
+int sdv2_attn_spans(const sdv2_view* q, const sdv2_view* k, const sdv2_view* v, const sdv2_view* out, int rows,
+                    int q_tokens, int heads, int head_dim, int64_t kv_tokens, const int32_t* begin_dev,
+                    int64_t begin_stride_row, int64_t begin_stride_tok, const int32_t* end_dev, int64_t end_stride_row,
+                    int64_t end_stride_tok, float softmax_scale, void* scratch_dev, size_t scratch_bytes,
+                    int* status_dev, void* stream);
+size_t sdv2_attn_spans_scratch_bytes(int rows, int q_tokens, int heads, int64_t kv_tokens);
+
 /* Synchronises `stream`, reads the status word at the start of a workspace and clears it.
  * Returns SDV2_OK, SDV2_ERR_TIMEOUT (a device-side wait ran out; *detail = where),
  * SDV2_ERR_INVALID_ARG (device-resident slot parameters were out of range; nothing was written) or

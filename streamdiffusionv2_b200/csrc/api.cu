@@ -62,6 +62,14 @@ int check_view(const sdv2_view* v, int esize, bool allow_row_broadcast) {
   return SDV2_OK;
 }
 
+// exponents of an 8-bit cache: bytes, so no alignment
+int check_exps(const sdv2_view* v, bool allow_row_broadcast) {
+  if (v == nullptr || v->ptr == nullptr) return SDV2_ERR_INVALID_ARG;
+  if (v->stride_tok <= 0 || v->stride_head <= 0) return SDV2_ERR_INVALID_ARG;
+  if (v->stride_row < 0 || (v->stride_row == 0 && !allow_row_broadcast)) return SDV2_ERR_INVALID_ARG;
+  return SDV2_OK;
+}
+
 PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
   static PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
     void* p = nullptr;
@@ -189,8 +197,8 @@ const char* sdv2_strerror(int code) {
 
 int sdv2_last_cuda_error(void) { return g_last_cuda_error; }
 
-// Shared by the two append entry points: slot parameters either in the four host arrays or in
-// `step_params_dev` (device, [4][rows]).
+// Shared by the append entry points: slot parameters either in the four host arrays or in `step_params_dev`
+// (device, [4][rows]); with k_exp / v_exp the caches are 8-bit ones.
 static int append_common(const sdv2_view* q, const sdv2_view* k, const sdv2_view* v, const sdv2_view* q_out,
                          const sdv2_view* k_cache, const sdv2_view* v_cache, int rows, int new_tokens, int heads,
                          int head_dim, int64_t cache_tokens, const double* rope_table_dev, int table_rows,
@@ -199,7 +207,7 @@ static int append_common(const sdv2_view* q, const sdv2_view* k, const sdv2_view
                          const int64_t* global_end_val, const int64_t* local_end_val,
                          const int64_t* step_params_dev, int dtype, int* status_dev, void* stream,
                          const void* norm_q_weight_dev = nullptr, const void* norm_k_weight_dev = nullptr,
-                         float norm_eps = 0.f) {
+                         float norm_eps = 0.f, const sdv2_view* k_exp = nullptr, const sdv2_view* v_exp = nullptr) {
   if (rows <= 0 || new_tokens <= 0 || heads <= 0 || cache_tokens <= 0 || table_rows <= 0) return SDV2_ERR_INVALID_ARG;
   if (grid_f <= 0 || grid_h <= 0 || grid_w <= 0) return SDV2_ERR_INVALID_ARG;
   if (static_cast<int64_t>(grid_f) * grid_h * grid_w != new_tokens) return SDV2_ERR_INVALID_ARG;
@@ -217,8 +225,12 @@ static int append_common(const sdv2_view* q, const sdv2_view* k, const sdv2_view
     return SDV2_ERR_INVALID_ARG;
   int rc;
   const sdv2_view* views[6] = {q, k, v, q_out, k_cache, v_cache};
-  for (const sdv2_view* vw : views)
-    if ((rc = check_view(vw, esize, false)) != SDV2_OK) return rc;
+  for (int i = 0; i < 6; ++i)
+    if ((rc = check_view(views[i], k_exp != nullptr && i >= 4 ? 1 : esize, false)) != SDV2_OK) return rc;
+  if (k_exp != nullptr) {
+    if (head_dim != 128) return SDV2_ERR_UNSUPPORTED_SHAPE;
+    if ((rc = check_exps(k_exp, false)) != SDV2_OK || (rc = check_exps(v_exp, false)) != SDV2_OK) return rc;
+  }
   if (grid_h > table_rows || grid_w > table_rows) return SDV2_ERR_INVALID_ARG;
   if ((norm_q_weight_dev == nullptr) != (norm_k_weight_dev == nullptr)) return SDV2_ERR_INVALID_ARG;
   if (norm_q_weight_dev != nullptr) {
@@ -262,6 +274,15 @@ static int append_common(const sdv2_view* q, const sdv2_view* k, const sdv2_view
   p.table_rows = table_rows;
   p.grid_f = grid_f;
   p.status = status_dev;
+  if (k_exp != nullptr) {
+    sdv2::Q8AppendParams qp;
+    memset(&qp, 0, sizeof(qp));
+    qp.a = p;
+    qp.k_exp = *k_exp;
+    qp.v_exp = *v_exp;
+    const cudaError_t qe = sdv2::launch_rope_kv_append_q8(qp, dtype, static_cast<cudaStream_t>(stream));
+    return qe == cudaSuccess ? SDV2_OK : cuda_fail(qe);
+  }
   cudaError_t e = sdv2::launch_rope_kv_append(p, dtype, static_cast<cudaStream_t>(stream));
   if (e == cudaErrorNotSupported) return SDV2_ERR_UNSUPPORTED_SHAPE;
   return e == cudaSuccess ? SDV2_OK : cuda_fail(e);
@@ -465,6 +486,164 @@ int sdv2_selftest_wait_timeout(int* status_dev, long long budget_cycles, void* s
   if (budget_cycles < 10000LL) budget_cycles = 10000LL;
   if (budget_cycles > 2000000000LL) budget_cycles = 2000000000LL;
   cudaError_t e = sdv2::launch_wait_timeout_selftest(status_dev, budget_cycles, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? SDV2_OK : cuda_fail(e);
+}
+
+// ------------------------------------------------------------------ 8-bit cache and key spans
+int sdv2_rope_kv_append_q8(const sdv2_view* q, const sdv2_view* k, const sdv2_view* v, const sdv2_view* q_out,
+                           const sdv2_view* k_cache, const sdv2_view* v_cache, const sdv2_view* k_exp,
+                           const sdv2_view* v_exp, int rows, int new_tokens, int heads, int head_dim,
+                           int64_t cache_tokens, const double* rope_table_dev, int table_rows, int grid_f, int grid_h,
+                           int grid_w, const int64_t* start_frame, const int64_t* dst_begin,
+                           const int64_t* step_params_dev, int64_t* global_end_dev, int64_t* local_end_dev,
+                           const int64_t* global_end_val, const int64_t* local_end_val, int dtype, int* status_dev,
+                           void* stream) {
+  if (k_exp == nullptr || v_exp == nullptr) return SDV2_ERR_INVALID_ARG;
+  return append_common(q, k, v, q_out, k_cache, v_cache, rows, new_tokens, heads, head_dim, cache_tokens,
+                       rope_table_dev, table_rows, grid_f, grid_h, grid_w, start_frame, dst_begin, global_end_dev,
+                       local_end_dev, global_end_val, local_end_val, step_params_dev, dtype, status_dev, stream, nullptr,
+                       nullptr, 0.f, k_exp, v_exp);
+}
+
+int sdv2_kv_read_q8(const sdv2_view* k_cache, const sdv2_view* v_cache, const sdv2_view* k_exp, const sdv2_view* v_exp,
+                    const sdv2_view* k_out, const sdv2_view* v_out, int rows, int tokens, int heads, int head_dim,
+                    int64_t cache_tokens, const int64_t* begin, int dtype, void* stream) {
+  if (rows <= 0 || tokens <= 0 || heads <= 0 || cache_tokens <= 0 || begin == nullptr) return SDV2_ERR_INVALID_ARG;
+  if (dtype != SDV2_DTYPE_BF16 && dtype != SDV2_DTYPE_F32) return SDV2_ERR_INVALID_ARG;
+  if (head_dim != 128 || rows > SDV2_MAX_ROWS) return SDV2_ERR_UNSUPPORTED_SHAPE;
+  int rc;
+  if ((rc = check_view(k_cache, 1, true)) != SDV2_OK || (rc = check_view(v_cache, 1, true)) != SDV2_OK) return rc;
+  if ((rc = check_exps(k_exp, true)) != SDV2_OK || (rc = check_exps(v_exp, true)) != SDV2_OK) return rc;
+  const int esize = dtype == SDV2_DTYPE_BF16 ? 2 : 4;
+  if ((rc = check_view(k_out, esize, false)) != SDV2_OK || (rc = check_view(v_out, esize, false)) != SDV2_OK) return rc;
+  sdv2::Q8ReadParams p;
+  memset(&p, 0, sizeof(p));
+  for (int b = 0; b < rows; ++b) {
+    if (begin[b] < 0 || begin[b] > cache_tokens - tokens) return SDV2_ERR_INVALID_ARG;
+    p.begin[b] = begin[b];
+  }
+  p.k = *k_cache; p.v = *v_cache; p.k_exp = *k_exp; p.v_exp = *v_exp; p.k_out = *k_out; p.v_out = *v_out;
+  p.rows = rows; p.tokens = tokens; p.heads = heads; p.dtype = dtype;
+  const cudaError_t e = sdv2::launch_kv_read_q8(p, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? SDV2_OK : cuda_fail(e);
+}
+
+static int fill_attn_x(sdv2::AttnXParams& p, int rows, int q_tokens, int heads, int64_t kv_tokens) {
+  if (rows <= 0 || q_tokens <= 0 || heads <= 0 || kv_tokens <= 0) return SDV2_ERR_INVALID_ARG;
+  if (rows > SDV2_MAX_ROWS || heads > 65535 || kv_tokens > 0x7FFFFF00LL || q_tokens > 0x7FFFFF00) return SDV2_ERR_UNSUPPORTED_SHAPE;
+  memset(&p, 0, sizeof(p));
+  p.rows = rows;
+  p.q_tokens = q_tokens;
+  p.heads = heads;
+  p.kv_tokens = static_cast<int>(kv_tokens);
+  p.pair_tiles = (q_tokens + 255) / 256;
+  if (static_cast<int64_t>(p.pair_tiles) * heads > 0x7FFFFFFFLL / 64 / rows) return SDV2_ERR_UNSUPPORTED_SHAPE;
+  return SDV2_OK;
+}
+
+static int plan_of(sdv2::AttnXParams& p, bool q8, int* slots) {
+  sdv2::DeviceInfo di;
+  const cudaError_t e = sdv2::device_info(&di);
+  if (e != cudaSuccess) return cuda_fail(e);
+  *slots = q8 ? sdv2::plan_q8(p, di.sms) : sdv2::plan_spans(p, di.sms);
+  return *slots < 0 ? SDV2_ERR_UNSUPPORTED_SHAPE : SDV2_OK;
+}
+
+static int fill_lens(sdv2::AttnXParams& p, const int32_t* seq_lens) {
+  if (seq_lens == nullptr) return SDV2_ERR_INVALID_ARG;
+  for (int b = 0; b < p.rows; ++b) {
+    if (seq_lens[b] < 0 || seq_lens[b] > p.kv_tokens) return SDV2_ERR_INVALID_ARG;
+    p.seq_lens[b] = seq_lens[b];
+  }
+  return SDV2_OK;
+}
+
+static int attn_x_common(sdv2::AttnXParams& p, bool q8, const sdv2_view* q, const sdv2_view* out, int head_dim,
+                         float softmax_scale, void* scratch, size_t scratch_bytes, int* status) {
+  if (head_dim != 128) return SDV2_ERR_UNSUPPORTED_SHAPE;
+  int rc;
+  if ((rc = check_view(q, 2, false)) != SDV2_OK || (rc = check_view(out, 2, false)) != SDV2_OK) return rc;
+  if (!(softmax_scale > 0.f) || !isfinite(softmax_scale)) return SDV2_ERR_INVALID_ARG;
+  p.out = out->ptr;
+  p.out_stride_row = out->stride_row;
+  p.out_stride_tok = out->stride_tok;
+  p.out_stride_head = out->stride_head;
+  p.scale_log2 = softmax_scale * 1.4426950408889634f;
+  p.status = status;
+  int slots = 0;
+  if ((rc = plan_of(p, q8, &slots)) != SDV2_OK) return rc;
+  if (slots > 0) {
+    if (scratch == nullptr || scratch_bytes < slots * sdv2::kAttnXPartFloats * sizeof(float)) return SDV2_ERR_WORKSPACE;
+    if (!aligned16(scratch)) return SDV2_ERR_MISALIGNED;
+    p.part_o = static_cast<float*>(scratch);
+    p.part_meta = p.part_o + static_cast<size_t>(slots) * 2 * 128 * 128;
+  }
+  return SDV2_OK;
+}
+
+size_t sdv2_attn_q8_scratch_bytes(int rows, int q_tokens, int heads, int64_t cache_tokens, const int32_t* seq_lens) {
+  sdv2::AttnXParams p;
+  int slots = 0;
+  if (fill_attn_x(p, rows, q_tokens, heads, cache_tokens) != SDV2_OK || fill_lens(p, seq_lens) != SDV2_OK ||
+      plan_of(p, true, &slots) != SDV2_OK)
+    return 0;
+  return slots * sdv2::kAttnXPartFloats * sizeof(float);
+}
+
+int sdv2_attn_kvcache_q8(const sdv2_view* q, const sdv2_view* k_cache, const sdv2_view* v_cache, const sdv2_view* k_exp,
+                         const sdv2_view* v_exp, const sdv2_view* out, int rows, int q_tokens, int heads, int head_dim,
+                         int64_t cache_tokens, const int32_t* seq_lens, float softmax_scale, void* scratch_dev,
+                         size_t scratch_bytes, int* status_dev, void* stream) {
+  sdv2::AttnXParams p;
+  int rc;
+  if ((rc = fill_attn_x(p, rows, q_tokens, heads, cache_tokens)) != SDV2_OK) return rc;
+  if ((rc = fill_lens(p, seq_lens)) != SDV2_OK) return rc;
+  if ((rc = check_view(k_cache, 1, true)) != SDV2_OK || (rc = check_view(v_cache, 1, true)) != SDV2_OK) return rc;
+  if ((rc = check_exps(k_exp, true)) != SDV2_OK || (rc = check_exps(v_exp, true)) != SDV2_OK) return rc;
+  if ((rc = attn_x_common(p, true, q, out, head_dim, softmax_scale, scratch_dev, scratch_bytes, status_dev)) != SDV2_OK)
+    return rc;
+  p.k = *k_cache; p.v = *v_cache; p.k_exp = *k_exp; p.v_exp = *v_exp;
+  CUtensorMap tm_q;
+  if ((rc = make_tile_map(&tm_q, q, rows, q_tokens, heads)) != SDV2_OK) return rc;
+  const cudaError_t e = sdv2::launch_attn_q8(tm_q, p, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? SDV2_OK : cuda_fail(e);
+}
+
+size_t sdv2_attn_spans_scratch_bytes(int rows, int q_tokens, int heads, int64_t kv_tokens) {
+  sdv2::AttnXParams p;
+  int slots = 0;
+  if (fill_attn_x(p, rows, q_tokens, heads, kv_tokens) != SDV2_OK || plan_of(p, false, &slots) != SDV2_OK) return 0;
+  return slots * sdv2::kAttnXPartFloats * sizeof(float);
+}
+
+int sdv2_attn_spans(const sdv2_view* q, const sdv2_view* k, const sdv2_view* v, const sdv2_view* out, int rows,
+                    int q_tokens, int heads, int head_dim, int64_t kv_tokens, const int32_t* begin_dev,
+                    int64_t begin_stride_row, int64_t begin_stride_tok, const int32_t* end_dev, int64_t end_stride_row,
+                    int64_t end_stride_tok, float softmax_scale, void* scratch_dev, size_t scratch_bytes,
+                    int* status_dev, void* stream) {
+  sdv2::AttnXParams p;
+  int rc;
+  if ((rc = fill_attn_x(p, rows, q_tokens, heads, kv_tokens)) != SDV2_OK) return rc;
+  if (end_dev == nullptr || (reinterpret_cast<uintptr_t>(end_dev) & 3u)) return SDV2_ERR_INVALID_ARG;
+  if (reinterpret_cast<uintptr_t>(begin_dev) & 3u) return SDV2_ERR_INVALID_ARG;
+  if (begin_stride_row < 0 || begin_stride_tok < 0 || end_stride_row < 0 || end_stride_tok < 0) return SDV2_ERR_INVALID_ARG;
+  if ((rc = check_view(k, 2, true)) != SDV2_OK || (rc = check_view(v, 2, true)) != SDV2_OK) return rc;
+  if ((k->stride_row == 0) != (v->stride_row == 0)) return SDV2_ERR_INVALID_ARG;
+  if ((rc = attn_x_common(p, false, q, out, head_dim, softmax_scale, scratch_dev, scratch_bytes, status_dev)) != SDV2_OK)
+    return rc;
+  p.kv_row_broadcast = k->stride_row == 0 ? 1 : 0;
+  p.begin = begin_dev;
+  p.end = end_dev;
+  p.begin_stride_row = begin_stride_row;
+  p.begin_stride_tok = begin_stride_tok;
+  p.end_stride_row = end_stride_row;
+  p.end_stride_tok = end_stride_tok;
+  const int kv_rows = p.kv_row_broadcast ? 1 : rows;
+  CUtensorMap tm_q, tm_k, tm_v;
+  if ((rc = make_tile_map(&tm_q, q, rows, q_tokens, heads)) != SDV2_OK) return rc;
+  if ((rc = make_tile_map(&tm_k, k, kv_rows, kv_tokens, heads)) != SDV2_OK) return rc;
+  if ((rc = make_tile_map(&tm_v, v, kv_rows, kv_tokens, heads)) != SDV2_OK) return rc;
+  const cudaError_t e = sdv2::launch_attn_spans(tm_q, tm_k, tm_v, p, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? SDV2_OK : cuda_fail(e);
 }
 

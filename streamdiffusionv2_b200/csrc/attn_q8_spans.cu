@@ -1,0 +1,764 @@
+// Attention over the 8-bit K/V cache, and attention in which every query has its own span of keys.
+//
+// Both run the loop of the bf16 cache kernel: one CTA per (pair of 128-row query tiles, head, row), one thread issues
+// S = Q K^T and O += P V (tcgen05, fp32 in TMEM), a softmax warpgroup per query tile, K/V through a ring of five
+// 32 KB tiles handed over as pairs (V_j, K_j+1), lazy rescaling of O.  What differs:
+//
+// kQ8.  K/V tiles are not copied by TMA: three warps load the cache's bytes into registers one tile ahead, expand them
+//   to bf16 and store them in the layout the tensor cores read.  A tile of K carries the largest exponent E of its
+//   tokens: it holds m * 2^(e-E-6), and 2^(E+6) joins the softmax scale of that tile, one multiplication per tile.  V
+//   tiles use R, the largest exponent of V so far, the same way; when R grows O is rescaled, as for a grown maximum.
+//   So a byte costs 1.5 instructions (permute, mask, multiply), the products see exactly the values the cache holds,
+//   and exponents may differ by 2^120 inside a head.
+//
+// Spans.  Row i attends keys [begin_i, end_i).  A CTA walks the key tiles between the smallest begin and the largest
+//   end of its rows; a thread masks its own row, and only in tiles that its span does not cover.  V rows that no row
+//   of the CTA attends are cleared on chip (0 x NaN would reach the output otherwise).  Rows with an empty span give 0.
+//
+// Split tiles write unnormalised O, the running maximum, sum and V exponent to scratch; combine_kernel merges them.
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "attn_tiles.cuh"
+#include "ptx.cuh"
+#include "q8.cuh"
+#include "sdv2_internal.h"
+
+namespace sdv2 {
+namespace attnx {
+
+using namespace attn;
+
+constexpr int kRing = 5;
+constexpr int kThreads = 384;
+constexpr int kExpandWarps = 3;
+constexpr uint32_t kSmemQ = 0;
+constexpr uint32_t kSmemKV = 2 * kTileBytes;
+constexpr uint32_t kSmemBar = kSmemKV + kRing * kTileBytes;
+constexpr uint32_t kSmemBytes = kSmemBar + 256 + 1024;  // + alignment slack
+constexpr uint32_t kTmemCols = 512;
+constexpr uint32_t kColS = 0, kColO = 256;
+
+constexpr int kPairBars = 3;
+constexpr int kBarQFull = 0;                       // [2]
+constexpr int kBarK0Full = 2;                      // K_0 in place
+constexpr int kBarPairFull = 3;                    // [kPairBars] V_g and K_{g+1} in place
+constexpr int kBarPairDone = 3 + kPairBars;        // [kPairBars] every MMA reading V_g or K_{g+1} (or older) completed
+constexpr int kBarSFull = 3 + 2 * kPairBars;       // [2]
+constexpr int kBarPFull = kBarSFull + 2;           // [2]
+constexpr int kBarOFull = kBarPFull + 2;           // [2]
+constexpr int kBarPHalf = kBarOFull + 2;           // [2] first 64 key columns of P written
+constexpr int kNumBars = kBarPHalf + 2;
+// words behind the barriers: abort flag, TMEM base, hull of the spans, exponents of the last four key tiles
+constexpr uint32_t kSmemWords = kSmemBar + kNumBars * 8;
+constexpr int kWordAbort = 0, kWordTmem = 1, kWordLo = 2, kWordHi = 3, kWordFullLo = 4, kWordFullHi = 5, kWordExpK = 6,
+              kWordExpV = 10, kNumWords = 14;
+static_assert(kNumBars * 8 + kNumWords * 4 <= 256, "barrier block too small");
+static_assert(kRing >= 5, "pair g overwrites the tiles of pairs g-3 and g-2: needs five slots");
+
+constexpr float kRescaleThreshold = 8.0f;  // log2 units
+
+__device__ __forceinline__ float exp2_int(int e) {  // 2^e, e clamped to fp32's normal range
+  return __int_as_float((min(max(e, -126), 127) + 127) << 23);
+}
+
+// ------------------------------------------------------------------ expanding the 8-bit cache (kQ8)
+// A tile is 32 groups of four tokens; expand warp w takes groups w, w + 3, ...  In a group a token has eight lanes of
+// 16 bytes each.
+constexpr int kGroups = (32 + kExpandWarps - 1) / kExpandWarps;
+
+struct TileBytes {
+  uint4 raw[kGroups];
+};
+
+// The lane's share of the 128 exponents of a tile: tokens lane, lane + 32, ... as four bytes.  Tokens past the end get
+// the smallest exponent.
+__device__ __forceinline__ uint32_t load_exps(const int8_t* base, int64_t stride_tok, int tok0, int seq_len, int lane) {
+  uint32_t packed = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int t = tok0 + i * 32 + lane;
+    const int e = t < seq_len ? base[static_cast<int64_t>(t) * stride_tok] : q8::kMinExp;
+    packed |= (static_cast<uint32_t>(e) & 0xFFu) << (8 * i);
+  }
+  return packed;
+}
+
+__device__ __forceinline__ int max_exp(uint32_t packed) {
+  int e = q8::kMinExp;  // vectors that are not finite carry -128 and leave it to the others
+#pragma unroll
+  for (int i = 0; i < 4; ++i) e = max(e, static_cast<int>(static_cast<int8_t>(packed >> (8 * i))));
+  return __reduce_max_sync(0xffffffffu, e);
+}
+
+__device__ __forceinline__ void load_bytes(TileBytes& t, const uint8_t* base, int64_t stride_tok, int tok0, int seq_len,
+                                           int w, int lane) {
+#pragma unroll
+  for (int i = 0; i < kGroups; ++i) {
+    const int g = i * kExpandWarps + w;
+    const int tok = tok0 + g * 4 + (lane >> 3);
+    t.raw[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (g < 32 && tok < seq_len)
+      t.raw[i] = __ldg(reinterpret_cast<const uint4*>(base + static_cast<int64_t>(tok) * stride_tok) + (lane & 7));
+  }
+}
+
+// Store the tile as bf16 m * 2^(e - ref - 6) in the 128-byte-swizzled layout of two 64-column halves.
+__device__ __forceinline__ void expand_tile(const TileBytes& t, uint32_t exps, int ref, uint8_t* tile, int w, int lane) {
+  const int c = lane & 7;
+  uint8_t* half = tile + (c >> 2) * kHalfTile;
+  const int ch = (2 * c) & 7;
+  const bool swap = c >= 4;  // the two halves store their chunks in opposite order: no bank is hit twice
+#pragma unroll
+  for (int i = 0; i < kGroups; ++i) {
+    const int g = i * kExpandWarps + w;
+    if (g >= 32) break;
+    const int tl = g * 4 + (lane >> 3);
+    const uint32_t ev = __shfl_sync(0xffffffffu, exps, tl & 31) >> (8 * (tl >> 5));
+    const int e = static_cast<int8_t>(ev);
+    // 2^(127 + e - ref) times the subnormal m * 2^-133; e <= ref, so the multiplier is a normal bf16 number
+    const uint32_t s2 = e == q8::kNotFinite ? 0x7FC07FC0u : static_cast<uint32_t>(254 + e - ref) * 0x00800080u;
+    const uint32_t in[4] = {t.raw[i].x, t.raw[i].y, t.raw[i].z, t.raw[i].w};
+    uint32_t o[8];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      q8::spread4(in[k], o[2 * k], o[2 * k + 1]);
+      o[2 * k] = q8::mul_bf16x2(o[2 * k], s2);
+      o[2 * k + 1] = q8::mul_bf16x2(o[2 * k + 1], s2);
+    }
+    const uint4 first = make_uint4(o[0], o[1], o[2], o[3]), second = make_uint4(o[4], o[5], o[6], o[7]);
+    uint8_t* row = half + tl * 128;
+    const int x = tl & 7;
+    *reinterpret_cast<uint4*>(row + (((swap ? ch + 1 : ch) ^ x) << 4)) = swap ? second : first;
+    *reinterpret_cast<uint4*>(row + (((swap ? ch : ch + 1) ^ x) << 4)) = swap ? first : second;
+  }
+}
+
+// ------------------------------------------------------------------ the kernel
+struct Item {
+  int b, h, q0, part, parts, slot;  // part < 0: the whole key range, written to the output directly
+};
+
+template <bool kQ8>
+__device__ __forceinline__ Item find_item(const AttnXParams& p, int i) {
+  Item it;
+  int pt, hb;
+  it.part = -1;
+  it.parts = 1;
+  it.slot = 0;
+  if (kQ8) {
+    int tile = i, r = 0;
+    if (i >= p.n_full) {
+      const int k = i - p.n_full;
+      r = p.rows - 1;
+      while (r > 0 && p.item0[r] > k) --r;
+      it.parts = p.parts[r];
+      const int local = k - p.item0[r];
+      tile = p.tail_tile0[r] + local / it.parts;
+      if (it.parts > 1) it.part = local % it.parts;
+      it.slot = k;
+    }
+    pt = tile % p.pair_tiles;
+    hb = tile / p.pair_tiles;
+    it.h = hb % p.heads;
+    it.b = p.order[hb / p.heads];
+  } else {
+    // late query tiles first: with masks that grow along the sequence they are the long ones
+    const int tile = i / p.split;
+    if (p.split > 1) it.part = i % p.split;
+    it.parts = p.split;
+    it.slot = i;
+    const int per = p.heads * p.rows;
+    pt = p.pair_tiles - 1 - tile / per;
+    hb = tile % per;
+    it.h = hb % p.heads;
+    it.b = hb / p.heads;
+  }
+  it.q0 = pt * (2 * kBM);
+  return it;
+}
+
+template <bool kQ8>
+__global__ void __launch_bounds__(kThreads, 1)
+attn_x_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+              const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ AttnXParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  uint8_t* gbase = smem_raw + (base - raw);
+  const uint32_t bar0 = base + kSmemBar;
+  auto bar = [&](int i) { return bar0 + 8u * i; };
+  volatile int* words = reinterpret_cast<volatile int*>(gbase + kSmemWords);
+  volatile int* abort_flag = words + kWordAbort;
+
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
+  const int lane = threadIdx.x & 31;
+  const Item item = find_item<kQ8>(p, blockIdx.x);
+  const int b = item.b, h = item.h, q0 = item.q0;
+  const bool two_tiles = q0 + kBM < p.q_tokens;
+  const int bk = p.kv_row_broadcast ? 0 : b;
+
+  if (threadIdx.x == 0) {
+    *abort_flag = 0;
+    words[kWordLo] = words[kWordFullHi] = 0x7FFFFFFF;
+    words[kWordHi] = words[kWordFullLo] = 0;
+    for (int i = 0; i < 2; ++i) mbar_init(bar(kBarQFull + i), 1);
+    mbar_init(bar(kBarK0Full), kQ8 ? kExpandWarps : 1);
+    for (int i = 0; i < kPairBars; ++i) {
+      mbar_init(bar(kBarPairFull + i), kQ8 ? kExpandWarps : 1);
+      mbar_init(bar(kBarPairDone + i), 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(bar(kBarSFull + i), 1);
+      mbar_init(bar(kBarPFull + i), kBM);
+      mbar_init(bar(kBarPHalf + i), kBM);
+      mbar_init(bar(kBarOFull + i), 1);
+    }
+    fence_mbar_init();
+    tma_prefetch_desc(&tm_q);
+    if (!kQ8) {
+      tma_prefetch_desc(&tm_k);
+      tma_prefetch_desc(&tm_v);
+    }
+  }
+  if (warp == 0) {
+    tmem_alloc(smem_u32(const_cast<int*>(words + kWordTmem)), kTmemCols);
+    tmem_relinquish();
+  }
+  // this thread's query row (softmax warps) and its span, clipped to the keys there are
+  int span_lo = 0, span_hi = 0;
+  const int my_row = q0 + (warp - 4) * 32 + lane;  // warps 4..11 are rows 0..255 of the tile pair
+  if (!kQ8 && warp >= 4 && my_row < p.q_tokens) {
+    const int64_t at = b * p.end_stride_row + static_cast<int64_t>(my_row) * p.end_stride_tok;
+    span_hi = min(p.end[at], p.kv_tokens);
+    if (p.begin != nullptr)
+      span_lo = max(p.begin[b * p.begin_stride_row + static_cast<int64_t>(my_row) * p.begin_stride_tok], 0);
+    if (span_lo >= span_hi) span_lo = span_hi = 0;
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (!kQ8) {
+    const bool some = span_hi > span_lo;
+    const int lo = __reduce_min_sync(0xffffffffu, some ? span_lo : 0x7FFFFFFF);
+    const int hi = __reduce_max_sync(0xffffffffu, some ? span_hi : 0);
+    const int flo = __reduce_max_sync(0xffffffffu, some ? span_lo : 0);
+    const int fhi = __reduce_min_sync(0xffffffffu, some ? span_hi : 0x7FFFFFFF);
+    if (warp >= 4 && lane == 0) {
+      atomicMin(const_cast<int*>(words + kWordLo), lo);
+      atomicMax(const_cast<int*>(words + kWordHi), hi);
+      atomicMax(const_cast<int*>(words + kWordFullLo), flo);
+      atomicMin(const_cast<int*>(words + kWordFullHi), fhi);
+    }
+    __syncthreads();
+  }
+  const uint32_t tmem = static_cast<uint32_t>(words[kWordTmem]);
+  // the keys that some row attends, the key tiles they lie in, and this item's share of those
+  const int key_lo = kQ8 ? 0 : words[kWordLo], key_hi = kQ8 ? p.seq_lens[b] : words[kWordHi];
+  const int tile_lo = kQ8 ? 0 : (key_lo < key_hi ? key_lo / kBN : 0);
+  const int n_kv_all = key_lo < key_hi ? (key_hi + kBN - 1) / kBN - tile_lo : 0;
+  const int j0 = tile_lo + (item.part < 0 ? 0 : static_cast<int>(static_cast<int64_t>(item.part) * n_kv_all / item.parts));
+  const int j1 = tile_lo + (item.part < 0 ? n_kv_all
+                                          : static_cast<int>(static_cast<int64_t>(item.part + 1) * n_kv_all / item.parts));
+  const int n_kv = j1 - j0;  // may be 0: nothing to attend
+
+  auto slot_off = [&](int it) { return kSmemKV + (it % kRing) * kTileBytes; };
+
+  if (warp == 0) {
+    // ------------------------------------------------------------------ MMA issuer
+    if (lane == 0 && n_kv > 0) {
+      const int n_stage = two_tiles ? 2 : 1;
+      for (int s = 0; s < n_stage; ++s) {
+        mbar_expect_tx(bar(kBarQFull + s), kTileBytes);
+        tma_load_4d(base + kSmemQ + s * kTileBytes, &tm_q, bar(kBarQFull + s), 0, h, q0 + s * kBM, b);
+        tma_load_4d(base + kSmemQ + s * kTileBytes + kHalfTile, &tm_q, bar(kBarQFull + s), 64, h, q0 + s * kBM, b);
+      }
+      const uint32_t sq[2] = {base + kSmemQ, base + kSmemQ + kTileBytes};
+      const uint32_t tS[2] = {tmem + kColS, tmem + kColS + 128};
+      const uint32_t tO[2] = {tmem + kColO, tmem + kColO + 128};
+      // Q first and unconditionally: this thread must not leave while its copies are in flight
+      bool ok = true;
+      for (int s = 0; s < n_stage; ++s) ok = mbar_wait(bar(kBarQFull + s), 0, abort_flag, p.status, WAIT_Q_FULL) && ok;
+      ok = ok && mbar_wait(bar(kBarK0Full), 0, abort_flag, p.status, WAIT_KV_FULL);
+      for (int s = 0; s < n_stage && ok; ++s) {
+        tc_fence_after();
+        issue_qk(tS[s], sq[s], base + slot_off(0));
+        umma_commit(bar(kBarSFull + s));
+      }
+      // step j: O += P_j V_j and S = Q K_{j+1}^T for each query tile; V_j and K_{j+1} are pair j of the ring
+      int slot_v = 1 % kRing, slot_k = 2 % kRing, pair_bar = 0, pair_par = 0;
+      for (int j = 0; j < n_kv && ok; ++j) {
+        const bool more = j + 1 < n_kv;
+        const uint32_t sv = base + kSmemKV + slot_v * kTileBytes, sk = base + kSmemKV + slot_k * kTileBytes;
+        for (int s = 0; s < n_stage && ok; ++s) {
+          ok = mbar_wait(bar(kBarPHalf + s), j & 1, abort_flag, p.status, WAIT_P_FULL);
+          if (ok && s == 0) ok = mbar_wait(bar(kBarPairFull + pair_bar), pair_par, abort_flag, p.status, WAIT_KV_FULL);
+          if (!ok) break;
+          tc_fence_after();
+          issue_pv(tO[s], tS[s], sv, j > 0, 0, 4);
+          ok = mbar_wait(bar(kBarPFull + s), j & 1, abort_flag, p.status, WAIT_P_FULL);
+          if (!ok) break;
+          tc_fence_after();
+          issue_pv(tO[s], tS[s], sv, true, 4, 8);
+          if (more) {
+            issue_qk(tS[s], sq[s], sk);
+            umma_commit(bar(kBarSFull + s));
+          } else {
+            umma_commit(bar(kBarOFull + s));
+          }
+        }
+        if (ok) umma_commit(bar(kBarPairDone + pair_bar));
+        slot_v = slot_v + 2 >= kRing ? slot_v + 2 - kRing : slot_v + 2;
+        slot_k = slot_k + 2 >= kRing ? slot_k + 2 - kRing : slot_k + 2;
+        if (++pair_bar == kPairBars) {
+          pair_bar = 0;
+          pair_par ^= 1;
+        }
+      }
+    }
+  } else if (warp < 4) {
+    if (kQ8) {
+      // ---------------------------------------------------------------- expand warps
+      const int w = warp - 1;
+      const uint8_t* kb = static_cast<const uint8_t*>(p.k.ptr) + bk * p.k.stride_row + h * p.k.stride_head;
+      const uint8_t* vb = static_cast<const uint8_t*>(p.v.ptr) + bk * p.v.stride_row + h * p.v.stride_head;
+      const int8_t* keb = static_cast<const int8_t*>(p.k_exp.ptr) + bk * p.k_exp.stride_row + h * p.k_exp.stride_head;
+      const int8_t* veb = static_cast<const int8_t*>(p.v_exp.ptr) + bk * p.v_exp.stride_row + h * p.v_exp.stride_head;
+      TileBytes rk, rv;
+      uint32_t ek = 0, ev = 0, ev_next = 0;
+      int ref_v = q8::kMinExp, ref_next = q8::kMinExp;
+      // K of a tile together with the exponents of its V, whose running maximum is published with K
+      auto load_k = [&](int g) {
+        const int tok0 = (j0 + g) * kBN;
+        ek = load_exps(keb, p.k_exp.stride_tok, tok0, key_hi, lane);
+        ev_next = load_exps(veb, p.v_exp.stride_tok, tok0, key_hi, lane);
+        load_bytes(rk, kb, p.k.stride_tok, tok0, key_hi, w, lane);
+      };
+      auto expand_k = [&](int g, int it) {
+        const int ref = max_exp(ek);
+        ref_next = max(ref_next, max_exp(ev_next));
+        if (w == 0 && lane == 0) {
+          words[kWordExpK + (g & 3)] = ref;
+          words[kWordExpV + (g & 3)] = ref_next;
+        }
+        expand_tile(rk, ek, ref, gbase + slot_off(it), w, lane);
+      };
+      auto arrive = [&](int i) {
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(i));
+      };
+      if (n_kv > 0) {
+        load_k(0);
+        load_bytes(rv, vb, p.v.stride_tok, j0 * kBN, key_hi, w, lane);
+        expand_k(0, 0);
+        arrive(kBarK0Full);
+      }
+      for (int g = 0; g < n_kv; ++g) {  // pair g = items 2g+1 (V_g) and 2g+2 (K_{g+1})
+        const bool more = g + 1 < n_kv;
+        ev = ev_next;
+        ref_v = ref_next;
+        if (more) load_k(g + 1);
+        // the slots of pair g held K_{g-2} and V_{g-2}: free once step g-2 of the issuer has completed
+        if (g >= 2) {
+          bool ok = mbar_wait(bar(kBarPairDone + (g - 2) % kPairBars), ((g - 2) / kPairBars) & 1, abort_flag, p.status,
+                              WAIT_KV_EMPTY);
+          if (!__all_sync(0xffffffffu, ok)) break;
+        }
+        expand_tile(rv, ev, ref_v, gbase + slot_off(2 * g + 1), w, lane);
+        if (more) {
+          load_bytes(rv, vb, p.v.stride_tok, (j0 + g + 1) * kBN, key_hi, w, lane);
+          expand_k(g + 1, 2 * g + 2);
+        }
+        arrive(kBarPairFull + g % kPairBars);
+      }
+    } else if (warp == 1 && lane == 0 && n_kv > 0) {
+      // ---------------------------------------------------------------- TMA producer
+      auto load_tile = [&](const CUtensorMap* tm, int it, int kv_tile, uint32_t full_bar) {
+        tma_load_4d(base + slot_off(it), tm, full_bar, 0, h, (j0 + kv_tile) * kBN, bk);
+        tma_load_4d(base + slot_off(it) + kHalfTile, tm, full_bar, 64, h, (j0 + kv_tile) * kBN, bk);
+      };
+      mbar_expect_tx(bar(kBarK0Full), kTileBytes);
+      load_tile(&tm_k, 0, 0, bar(kBarK0Full));
+      bool ok = true;
+      int issued = 0;  // pairs requested
+      for (int g = 0; g < n_kv; ++g) {
+        if (g >= 2)
+          ok = mbar_wait(bar(kBarPairDone + (g - 2) % kPairBars), ((g - 2) / kPairBars) & 1, abort_flag, p.status,
+                         WAIT_KV_EMPTY);
+        if (!ok) break;
+        const bool more = g + 1 < n_kv;
+        const uint32_t full = bar(kBarPairFull + g % kPairBars);
+        mbar_expect_tx(full, more ? 2 * kTileBytes : kTileBytes);
+        load_tile(&tm_v, 2 * g + 1, g, full);
+        if (more) load_tile(&tm_k, 2 * g + 2, g + 1, full);
+        issued = g + 1;
+      }
+      if (!ok) {
+        // leave no copy in flight: wait (bounded) for the tiles already requested
+        const long long t0 = clock64();
+        while (!mbar_try_wait(bar(kBarK0Full), 0) && clock64() - t0 < kWaitBudgetCycles) {
+        }
+        for (int g = (issued > kPairBars ? issued - kPairBars : 0); g < issued; ++g) {
+          const long long t1 = clock64();
+          while (!mbar_try_wait(bar(kBarPairFull + g % kPairBars), (g / kPairBars) & 1) &&
+                 clock64() - t1 < kWaitBudgetCycles) {
+          }
+        }
+      }
+    }
+  } else {
+    // ------------------------------------------------------------------ softmax + epilogue
+    const int stage = (warp - 4) >> 2;
+    if (stage == 0 || two_tiles) {
+      const int quad = warp & 3;
+      const int row = quad * 32 + lane;
+      const uint32_t lane_base = static_cast<uint32_t>(quad * 32) << 16;
+      const uint32_t tS = tmem + lane_base + kColS + stage * 128;
+      const uint32_t tO = tmem + lane_base + kColO + stage * 128;
+      const int full_lo = kQ8 ? 0 : words[kWordFullLo], full_hi = kQ8 ? key_hi : words[kWordFullHi];
+      float m_used = -INFINITY;  // running maximum (lags by up to the threshold); -inf: no key so far
+      float l = 0.f;
+      int ref_v = 0;  // V exponent the accumulator is in (kQ8)
+      bool ok = true;
+      for (int j = 0; j < n_kv; ++j) {
+        ok = mbar_wait(bar(kBarSFull + stage), j & 1, abort_flag, p.status, WAIT_S_FULL);
+        if (kQ8 && ok)  // K_j's and V_j's exponents were published with K_j: already complete, read for its ordering
+          ok = j == 0 ? mbar_wait(bar(kBarK0Full), 0, abort_flag, p.status, WAIT_KV_FULL)
+                      : mbar_wait(bar(kBarPairFull + (j - 1) % kPairBars), ((j - 1) / kPairBars) & 1, abort_flag, p.status,
+                                  WAIT_KV_FULL);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+        uint32_t s[4][32];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld32(tS + c * 32, s[c]);
+        tmem_wait_ld();
+        const int key0 = (j0 + j) * kBN;
+        const int lo = kQ8 ? 0 : span_lo - key0, hi = (kQ8 ? key_hi : span_hi) - key0;
+        if (lo > 0 || hi < kBN) {
+          const uint32_t width = static_cast<uint32_t>(max(hi - lo, 0));
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (static_cast<uint32_t>(c * 32 + i - lo) >= width) s[c][i] = 0xFF800000u;  // -inf
+        }
+        // V rows that no query row of this CTA attends lie inside the tensor, so the TMA did not zero-fill them and they
+        // may hold anything, NaN included; P is 0 there, but 0 x NaN would poison output rows.  Query tile 0 clears
+        // them in shared memory before it reports P (tile 1's P V is issued later).  (kQ8: expanded as zeros.)
+        if (!kQ8 && stage == 0 && (key0 < full_lo || key0 + kBN > full_hi)) {
+          ok = mbar_wait(bar(kBarPairFull + j % kPairBars), (j / kPairBars) & 1, abort_flag, p.status, WAIT_KV_FULL);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          const int key = key0 + row;
+          const bool in_hull = key >= key_lo && key < key_hi;
+          bool attended = false;
+          // rows in a scattered order, so that a few of them usually settle it
+          for (int i = 0; i < 2 * kBM && __any_sync(0xffffffffu, in_hull && !attended); ++i) {
+            const int r = q0 + ((i * 97) & (2 * kBM - 1));
+            if (r >= p.q_tokens) continue;
+            const int e = p.end[b * p.end_stride_row + static_cast<int64_t>(r) * p.end_stride_tok];
+            const int a = p.begin == nullptr ? 0 : p.begin[b * p.begin_stride_row + static_cast<int64_t>(r) * p.begin_stride_tok];
+            attended = attended || (key >= a && key < e);
+          }
+          if (!(in_hull && attended)) {
+            uint8_t* vrow = gbase + slot_off(2 * j + 1) + row * 128;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              *reinterpret_cast<uint4*>(vrow + 16 * i) = make_uint4(0u, 0u, 0u, 0u);
+              *reinterpret_cast<uint4*>(vrow + kHalfTile + 16 * i) = make_uint4(0u, 0u, 0u, 0u);
+            }
+          }
+          fence_proxy_async_smem();
+        }
+        float mx0 = -INFINITY, mx1 = -INFINITY, mx2 = -INFINITY, mx3 = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int i = 0; i < 32; i += 4) {
+            mx0 = fmaxf(mx0, __uint_as_float(s[c][i]));
+            mx1 = fmaxf(mx1, __uint_as_float(s[c][i + 1]));
+            mx2 = fmaxf(mx2, __uint_as_float(s[c][i + 2]));
+            mx3 = fmaxf(mx3, __uint_as_float(s[c][i + 3]));
+          }
+        float scale = p.scale_log2;
+        int ref_new = 0;
+        if (kQ8) {
+          scale = fmaxf(scale * exp2_int(words[kWordExpK + (j & 3)] + 6), 1.17549435e-38f);
+          ref_new = words[kWordExpV + (j & 3)];
+        }
+        const float mx = fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3)) * scale;
+        if (j == 0) {
+          m_used = mx;
+          ref_v = ref_new;
+        } else {
+          const bool grow = mx > m_used + kRescaleThreshold;
+          const bool shift = kQ8 && ref_new != ref_v;  // the same for every row
+          if (__any_sync(0xffffffffu, grow || shift)) {
+            const float m_new = grow ? mx : m_used;
+            float alpha = grow ? ex2_approx(m_used - m_new) : 1.f;
+            m_used = m_new;
+            l *= alpha;
+            if (kQ8) alpha *= exp2_int(ref_v - ref_new);
+            ref_v = ref_new;
+            // O of this stage is idle here: P V of the previous kv tile completed before S arrived
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c) {
+              uint32_t o[32];
+              tmem_ld32(tO + c * 32, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+              tmem_st32(tO + c * 32, o);
+            }
+          }
+        }
+        const float m_sub = m_used == -INFINITY ? 0.f : m_used;  // no key yet: exponentials of -inf, not of -inf + inf
+        float sum0 = 0.f, sum1 = 0.f;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float p0 = ex2_approx(fmaf(__uint_as_float(s[c][2 * i]), scale, -m_sub));
+            const float p1 = ex2_approx(fmaf(__uint_as_float(s[c][2 * i + 1]), scale, -m_sub));
+            sum0 += p0;
+            sum1 += p1;
+            pk[i] = pack_bf16x2(p0, p1);
+          }
+          tmem_st16(tS + c * 16, pk);
+          if (c == 1) {  // the first 64 keys of P are complete: their share of P V can start
+            tmem_wait_st();
+            tc_fence_before();
+            mbar_arrive(bar(kBarPHalf + stage));
+          }
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(bar(kBarPFull + stage));
+        l += sum0 + sum1;
+      }
+      if (ok && n_kv > 0) {
+        ok = mbar_wait(bar(kBarOFull + stage), 0, abort_flag, p.status, WAIT_O_FULL);
+        ok = __all_sync(0xffffffffu, ok);
+        tc_fence_after();
+      }
+      if (ok && item.part < 0) {
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const float unit = kQ8 ? exp2_int(ref_v + 6) : 1.f;
+        const int q_row = q0 + stage * kBM + row;
+        __nv_bfloat16* op = static_cast<__nv_bfloat16*>(p.out) + static_cast<int64_t>(b) * p.out_stride_row +
+                            static_cast<int64_t>(q_row) * p.out_stride_tok +
+                            static_cast<int64_t>(h) * p.out_stride_head;
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+          uint32_t o[32];
+          if (n_kv > 0) {
+            tmem_ld32(tO + c * 32, o);
+            tmem_wait_ld();
+          }
+          if (q_row < p.q_tokens) {
+            float y[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              y[i] = l == 0.f ? 0.f : __uint_as_float(o[i]) * inv;
+              if (kQ8) y[i] *= unit;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              uint4 v;
+              v.x = pack_bf16x2(y[8 * i + 0], y[8 * i + 1]);
+              v.y = pack_bf16x2(y[8 * i + 2], y[8 * i + 3]);
+              v.z = pack_bf16x2(y[8 * i + 4], y[8 * i + 5]);
+              v.w = pack_bf16x2(y[8 * i + 6], y[8 * i + 7]);
+              *reinterpret_cast<uint4*>(op + c * 32 + i * 8) = v;
+            }
+          }
+        }
+      } else if (ok) {
+        // partial result of one key range: unnormalised accumulator, running maximum and sum, V exponent
+        float* po = p.part_o + (static_cast<size_t>(item.slot) * 2 + stage) * (kBM * kHD) + row * kHD;
+        float* pm = p.part_meta + (static_cast<size_t>(item.slot) * 2 + stage) * (3 * kBM);
+        pm[row] = m_used;
+        pm[kBM + row] = l;
+        pm[2 * kBM + row] = static_cast<float>(ref_v);
+        if (n_kv > 0) {
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            uint32_t o[32];
+            tmem_ld32(tO + c * 32, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              *reinterpret_cast<uint4*>(po + c * 32 + i * 4) =
+                  make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+          }
+        }
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 0) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kTmemCols);
+  }
+}
+
+// Merge the parts of the split tiles.  Block = (split tile, query tile, group of 32 rows); 256 threads = 32 rows x 8
+// column groups of 16.  out = sum_k w_k O_k / sum_k 2^(m_k - m) l_k with w_k = 2^(m_k - m + R_k - R) and the result in
+// units of 2^(R+6); a part without a key has l_k = 0 and no accumulator.
+template <bool kQ8>
+__global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ AttnXParams p) {
+  const int stage = blockIdx.y;
+  const int row = blockIdx.z * 32 + (threadIdx.x >> 3);
+  const int c0 = (threadIdx.x & 7) * 16;
+  int first;
+  if (kQ8) {  // the first item of the blockIdx.x-th tail tile
+    const int tile = p.n_full + blockIdx.x;
+    int r = p.rows - 1;
+    while (r > 0 && p.tail_tile0[r] > tile) --r;
+    first = p.n_full + p.item0[r] + (tile - p.tail_tile0[r]) * p.parts[r];
+  } else {
+    first = blockIdx.x * p.split;
+  }
+  const Item item = find_item<kQ8>(p, first);
+  const int q_row = item.q0 + stage * kBM + row;
+  if (item.part < 0 || q_row >= p.q_tokens) return;
+  const float* pm = p.part_meta + (static_cast<size_t>(item.slot) * 2 + stage) * (3 * kBM) + row;
+  const float* po = p.part_o + (static_cast<size_t>(item.slot) * 2 + stage) * (kBM * kHD) + row * kHD + c0;
+  constexpr size_t pm_step = 2 * 3 * kBM, po_step = static_cast<size_t>(2) * kBM * kHD;
+  float m = -INFINITY, ref = q8::kMinExp;
+  for (int k = 0; k < item.parts; ++k) {
+    m = fmaxf(m, pm[k * pm_step]);
+    if (kQ8 && pm[k * pm_step + kBM] != 0.f) ref = fmaxf(ref, pm[k * pm_step + 2 * kBM]);
+  }
+  const float m_sub = m == -INFINITY ? 0.f : m;
+  float l = 0.f;
+  float acc[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) acc[i] = 0.f;
+  for (int k = 0; k < item.parts; ++k) {
+    const float lk = pm[k * pm_step + kBM];
+    if (lk == 0.f) continue;
+    const float up = exp2f(pm[k * pm_step] - m_sub);
+    const float w = kQ8 ? up * exp2_int(static_cast<int>(pm[k * pm_step + 2 * kBM] - ref)) : up;
+    l += up * lk;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float4 a = *reinterpret_cast<const float4*>(po + k * po_step + 4 * i);
+      acc[4 * i + 0] += w * a.x; acc[4 * i + 1] += w * a.y; acc[4 * i + 2] += w * a.z; acc[4 * i + 3] += w * a.w;
+    }
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const float unit = kQ8 ? exp2_int(static_cast<int>(ref) + 6) : 1.f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) acc[i] = acc[i] * inv * unit;
+  __nv_bfloat16* op = static_cast<__nv_bfloat16*>(p.out) + static_cast<int64_t>(item.b) * p.out_stride_row +
+                      static_cast<int64_t>(q_row) * p.out_stride_tok +
+                      static_cast<int64_t>(item.h) * p.out_stride_head + c0;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    *reinterpret_cast<uint4*>(op + 8 * i) =
+        make_uint4(pack_bf16x2(acc[8 * i + 0], acc[8 * i + 1]), pack_bf16x2(acc[8 * i + 2], acc[8 * i + 3]),
+                   pack_bf16x2(acc[8 * i + 4], acc[8 * i + 5]), pack_bf16x2(acc[8 * i + 6], acc[8 * i + 7]));
+}
+
+template <bool kQ8>
+cudaError_t launch(const CUtensorMap& tm_q, const CUtensorMap& tm_k, const CUtensorMap& tm_v, const AttnXParams& p,
+                   cudaStream_t stream) {
+  static DynamicSmemGrant smem_grant;  // one per instantiation
+  DeviceInfo di;
+  cudaError_t e = device_info(&di);
+  if (e == cudaSuccess) e = smem_grant.ensure(attn_x_kernel<kQ8>, static_cast<int>(kSmemBytes), di.device);
+  if (e != cudaSuccess) return e;
+  const int items = kQ8 ? p.n_full + p.n_parts : p.n_tiles * p.split;
+  attn_x_kernel<kQ8><<<items, kThreads, kSmemBytes, stream>>>(tm_q, tm_k, tm_v, p);
+  e = cudaGetLastError();
+  const int merged = kQ8 ? (p.split > 1 ? p.n_tiles - p.n_full : 0) : (p.split > 1 ? p.n_tiles : 0);
+  if (e != cudaSuccess || merged == 0) return e;
+  combine_kernel<kQ8><<<dim3(merged, p.q_tokens > kBM ? 2 : 1, kBM / 32), 256, 0, stream>>>(p);
+  return cudaGetLastError();
+}
+
+}  // namespace attnx
+
+cudaError_t launch_attn_q8(const CUtensorMap& tm_q, const AttnXParams& p, cudaStream_t stream) {
+  return attnx::launch<true>(tm_q, tm_q, tm_q, p, stream);
+}
+
+cudaError_t launch_attn_spans(const CUtensorMap& tm_q, const CUtensorMap& tm_k, const CUtensorMap& tm_v,
+                              const AttnXParams& p, cudaStream_t stream) {
+  return attnx::launch<false>(tm_q, tm_k, tm_v, p, stream);
+}
+
+// Splitting along the keys.  With one CTA per SM, n_tiles = waves * sms + tail leaves only `tail` SMs busy at the end
+// (all of them, when there are few tiles).  The tail's tiles - those of the shortest rows, rows are taken longest first -
+// are cut into parts of about c key tiles, c the smallest for which the parts still fit one wave.  A part costs its
+// set-up and a pass over its accumulator, so c stays at kMinTiles or more.
+int plan_q8(AttnXParams& p, int sms) {
+  constexpr int kMinTiles = 8;
+  const int per_row = p.pair_tiles * p.heads;
+  int n_kv[SDV2_MAX_ROWS], first[SDV2_MAX_ROWS];
+  for (int r = 0; r < p.rows; ++r) {  // insertion sort, longest row first
+    int at = r;
+    while (at > 0 && p.seq_lens[p.order[at - 1]] < p.seq_lens[r]) {
+      p.order[at] = p.order[at - 1];
+      --at;
+    }
+    p.order[at] = r;
+  }
+  const int64_t n_tiles = static_cast<int64_t>(per_row) * p.rows;
+  if (n_tiles > 0x7FFFFFFFLL / 64) return -1;
+  p.n_tiles = static_cast<int>(n_tiles);
+  p.n_full = p.n_tiles - p.n_tiles % sms;
+  int longest = 0;
+  for (int r = 0; r < p.rows; ++r) {
+    n_kv[r] = (p.seq_lens[p.order[r]] + 127) / 128;
+    first[r] = max(r * per_row, p.n_full);
+    if ((r + 1) * per_row > p.n_full) longest = max(longest, n_kv[r]);
+  }
+  auto parts_at = [&](int c, int r) { return n_kv[r] <= c ? 1 : (n_kv[r] + c - 1) / c; };
+  auto items_at = [&](int c) {
+    int64_t n = 0;
+    for (int r = 0; r < p.rows; ++r) n += static_cast<int64_t>(max((r + 1) * per_row - first[r], 0)) * parts_at(c, r);
+    return n;
+  };
+  int lo = kMinTiles, hi = max(longest, kMinTiles);  // the smallest c in [lo, hi] whose parts fit; hi always does
+  while (lo < hi) {
+    const int c = (lo + hi) / 2;
+    if (items_at(c) <= sms) hi = c;
+    else lo = c + 1;
+  }
+  p.split = 1;
+  int item = 0;
+  for (int r = 0; r < p.rows; ++r) {
+    p.tail_tile0[r] = first[r];
+    p.item0[r] = item;
+    p.parts[r] = parts_at(lo, r);
+    const int tiles = max((r + 1) * per_row - first[r], 0);
+    if (tiles > 0) p.split = max(p.split, p.parts[r]);
+    item += tiles * p.parts[r];
+  }
+  p.n_parts = item;
+  return p.split > 1 ? p.n_parts : 0;
+}
+
+// Spans live on the device, so the host splits by the number of tiles and keys alone: parts whose share is empty cost
+// little.
+int plan_spans(AttnXParams& p, int sms) {
+  constexpr int kMinTiles = 4;
+  const int64_t n_tiles = static_cast<int64_t>(p.pair_tiles) * p.heads * p.rows;
+  if (n_tiles > 0x7FFFFFFFLL / 64) return -1;
+  p.n_tiles = static_cast<int>(n_tiles);
+  p.split = 1;
+  if (p.n_tiles < sms) p.split = max(1, min(min(sms / p.n_tiles, 64), (p.kv_tokens + 127) / 128 / kMinTiles));
+  return p.split > 1 ? p.n_tiles * p.split : 0;
+}
+
+}  // namespace sdv2

@@ -153,6 +153,54 @@ int record_cuda_error(cudaError_t e);
 cudaError_t launch_attn_tcgen05(const CUtensorMap& tm_q, const CUtensorMap& tm_k, const CUtensorMap& tm_v,
                                 const AttnParams& p, cudaStream_t stream);
 
+// Append into the 8-bit cache: `a` with k_cache / v_cache as byte tensors, plus the exponents beside them.
+struct Q8AppendParams {
+  AppendParams a;
+  sdv2_view k_exp, v_exp;
+  int head_groups, heads_per_group;  // filled in by the launcher: warps per token, heads of each
+};
+cudaError_t launch_rope_kv_append_q8(const Q8AppendParams& p, int dtype, cudaStream_t stream);
+
+struct Q8ReadParams {
+  sdv2_view k, v, k_exp, v_exp, k_out, v_out;
+  int rows, tokens, heads, dtype;
+  int row_vecs, block_tokens;  // filled in by the launcher
+  uint32_t magic_row_vecs;
+  int64_t begin[SDV2_MAX_ROWS];
+};
+cudaError_t launch_kv_read_q8(const Q8ReadParams& p, cudaStream_t stream);
+
+// Attention over the 8-bit cache and attention over key spans (attn_q8_spans.cu).
+struct AttnXParams {
+  void* out;
+  int64_t out_stride_row, out_stride_tok, out_stride_head;  // elements
+  int rows, q_tokens, heads, kv_tokens;
+  int kv_row_broadcast;  // 1: every row reads K/V row 0
+  float scale_log2;      // softmax_scale * log2(e)
+  int* status;
+  float* part_o;         // [parts][2][128][128] fp32
+  float* part_meta;      // [parts][2][3][128] fp32: running maximum (log2 units), sum, V exponent
+  int pair_tiles, n_tiles;
+  int split;             // spans: parts of every tile; 8-bit cache: the most parts of a tile
+  // 8-bit cache: rows longest first; tiles [0, n_full) whole, the others in parts[r] parts, n_parts items in all
+  sdv2_view k, v, k_exp, v_exp;
+  int n_full, n_parts;
+  int seq_lens[SDV2_MAX_ROWS];     // by row
+  int order[SDV2_MAX_ROWS];        // rows, longest first; the arrays below go by place in this order
+  int tail_tile0[SDV2_MAX_ROWS], item0[SDV2_MAX_ROWS], parts[SDV2_MAX_ROWS];
+  // spans
+  const int* begin;  // null: 0
+  const int* end;
+  int64_t begin_stride_row, begin_stride_tok, end_stride_row, end_stride_tok;
+};
+constexpr size_t kAttnXPartFloats = 2 * (128 * 128 + 3 * 128);
+// Fill in how the work is cut up; returns the partial-result slots needed (0: none) or -1 (too many tiles).
+int plan_q8(AttnXParams& p, int sms);
+int plan_spans(AttnXParams& p, int sms);
+cudaError_t launch_attn_q8(const CUtensorMap& tm_q, const AttnXParams& p, cudaStream_t stream);
+cudaError_t launch_attn_spans(const CUtensorMap& tm_q, const CUtensorMap& tm_k, const CUtensorMap& tm_v,
+                              const AttnXParams& p, cudaStream_t stream);
+
 struct SimtAttnParams {
   sdv2_view q, k, v, out;
   int rows, q_tokens, heads;

@@ -5,6 +5,7 @@ not synchronise.  There is no CPU or PyTorch fallback: a missing library or a fa
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import math
 from typing import Dict, Optional, Sequence, Tuple
@@ -297,6 +298,196 @@ def attn_kvcache_simt(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
                                         N.i32_array(seq_lens), scale, N.dtype_code(q.dtype),
                                         N.stream_ptr(q.device))
     N.check(rc, "sdv2_attn_kvcache_simt")
+    return out
+
+
+def _on_device(t: torch.Tensor):
+    """Context in which a launch goes to `t`'s device, whatever the current one is."""
+    idx = t.device.index
+    return contextlib.nullcontext() if idx == torch.cuda.current_device() else torch.cuda.device(idx)
+
+
+def _check_same(what: str, ref: torch.Tensor, tensors: dict) -> None:
+    for name, (t, shape, dtype) in tensors.items():
+        if tuple(t.shape) != tuple(shape) or t.dtype != dtype or t.device != ref.device:
+            raise ValueError(f"{what}: {name} must be a {dtype} tensor {list(shape)} on {ref.device}, "
+                             f"not {t.dtype} {list(t.shape)} on {t.device}")
+
+
+def _exp_view(t: torch.Tensor) -> N.View:
+    """[rows, tokens, heads] int8 exponents of an 8-bit cache (a size-1 dimension may carry any stride: give it a legal
+    one)."""
+    tok, head = t.stride(1) if t.shape[1] > 1 else max(1, t.shape[2]), t.stride(2) if t.shape[2] > 1 else 1
+    return N.View(t.data_ptr(), t.stride(0) if t.shape[0] > 1 else t.shape[1] * tok, tok, head)
+
+
+def _check_q8(what: str, ref: torch.Tensor, k_cache, v_cache, k_exp, v_exp, rows: int, heads: int, head_dim: int) -> int:
+    """Shapes, types and devices of an 8-bit cache's four tensors; returns its length in tokens."""
+    if head_dim != 128:
+        raise ValueError(f"{what}: the 8-bit cache has head_dim 128, not {head_dim}")
+    smax = k_cache.shape[1] if k_cache.dim() == 4 else 0
+    shape = (rows, smax, heads, head_dim)
+    _check_same(what, ref, {"k_cache": (k_cache, shape, torch.uint8), "v_cache": (v_cache, shape, torch.uint8),
+                            "k_exp": (k_exp, shape[:3], torch.int8), "v_exp": (v_exp, shape[:3], torch.int8)})
+    return smax
+
+
+def q8_cache(rows: int, tokens: int, heads: int, device) -> Dict[str, torch.Tensor]:
+    """The four tensors of an 8-bit K/V cache, holding zeros: "k", "v" uint8 [rows, tokens, heads, 128] and "k_exp",
+    "v_exp" int8 [rows, tokens, heads].  A head vector holds sign * magnitude * 2^exponent, the sign in a byte's top
+    bit; see `rope_kv_append_q8`."""
+    shape = (rows, tokens, heads, 128)
+    out = {n: torch.zeros(shape, dtype=torch.uint8, device=device) for n in ("k", "v")}
+    out.update({n: torch.zeros(shape[:3], dtype=torch.int8, device=device) for n in ("k_exp", "v_exp")})
+    return out
+
+
+def rope_kv_append_q8(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                      k_exp: torch.Tensor, v_exp: torch.Tensor, table: torch.Tensor, grid: Sequence[int],
+                      start_frames: Sequence[int], dst_begin: Sequence[int], *, q_out: Optional[torch.Tensor] = None,
+                      index_tensors: Optional[Tuple[torch.Tensor, torch.Tensor]] = None,
+                      index_values: Optional[Tuple[Sequence[int], Sequence[int]]] = None,
+                      step_params: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """`rope_kv_append` into an 8-bit cache (`q8_cache`): ropes q and k and writes k / v of every row into cache slot
+    [dst_begin[b], dst_begin[b] + N), one power-of-two exponent per (token, head): e = max(floor(log2(max|x|)) - 6, -126),
+    magnitudes min(rint(|x| / 2^e), 127).  A head vector with a value that is not finite reads back as NaN.
+    q, k, v [B, N, H, 128] bf16 or fp32; `index_tensors`, `index_values`, `step_params` as for `rope_kv_append`.
+    Returns the roped q, the same bits as `rope_kv_append`'s."""
+    B, n_new, H, D = q.shape
+    smax = _check_q8("rope_kv_append_q8", q, k_cache, v_cache, k_exp, v_exp, B, H, D)
+    if q_out is None:
+        q_out = torch.empty((B, n_new, H, D), dtype=q.dtype, device=q.device)
+    _check_same("rope_kv_append_q8", q, {"k": (k, q.shape, q.dtype), "v": (v, q.shape, q.dtype),
+                                         "q_out": (q_out, q.shape, q.dtype),
+                                         "table": (table, (table.shape[0], D // 2, 2), torch.float64)})
+    if not table.is_contiguous():
+        raise ValueError("rope_kv_append_q8: the rope table must be contiguous")
+    f, h, w = (int(x) for x in grid)
+    ge_dev = le_dev = ge_val = le_val = params = None
+    if index_tensors is not None:
+        g, l = index_tensors
+        for t in (g, l):
+            if t.dtype != torch.int64 or t.numel() < B or not t.is_contiguous() or t.device != q.device:
+                raise ValueError("index tensors must be contiguous int64 with one entry per row, on q's device")
+        ge_dev, le_dev = g.data_ptr(), l.data_ptr()
+    starts = dsts = None
+    if step_params is not None:
+        if (step_params.dtype != torch.int64 or not step_params.is_contiguous() or step_params.numel() != 4 * B
+                or step_params.device != q.device):
+            raise ValueError("step_params must be a contiguous int64 [4, rows] tensor on the same device")
+        params = step_params.data_ptr()
+    else:
+        if len(start_frames) < B or len(dst_begin) < B:
+            raise ValueError("start_frames and dst_begin need one entry per row")
+        starts, dsts = N.i64_array(start_frames), N.i64_array(dst_begin)
+        if index_tensors is not None:
+            if index_values is None or len(index_values[0]) < B or len(index_values[1]) < B:
+                raise ValueError("index_values need one entry per row")
+            ge_val, le_val = N.i64_array(index_values[0]), N.i64_array(index_values[1])
+    views = [N.view(t) for t in (q, k, v, q_out, k_cache, v_cache)] + [_exp_view(k_exp), _exp_view(v_exp)]
+    args = [*[C.byref(x) for x in views], B, n_new, H, D, smax, table.data_ptr(), table.shape[0], f, h, w, starts, dsts,
+            params, ge_dev, le_dev, ge_val, le_val, N.dtype_code(q.dtype), workspace(q.device).data_ptr(),
+            N.stream_ptr(q.device)]
+    fn = N.lib().sdv2_rope_kv_append_q8
+    with _on_device(q), _Logged("rope_kv_append_q8", B * n_new * H * (4.0 * D * q.element_size() + 2 * (D + 1))):
+        rc = fn(*args)
+    N.check(rc, "sdv2_rope_kv_append_q8")
+    return q_out
+
+
+def kv_read_q8(k_cache: torch.Tensor, v_cache: torch.Tensor, k_exp: torch.Tensor, v_exp: torch.Tensor,
+               begin: Sequence[int], tokens: int, *, dtype: torch.dtype = torch.bfloat16,
+               out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(k, v) [B, tokens, H, 128]: what an 8-bit cache holds of tokens begin[b] .. begin[b] + tokens - 1 of every row,
+    in bf16 or fp32 (both exact)."""
+    B, _, H, D = k_cache.shape
+    smax = _check_q8("kv_read_q8", k_cache, k_cache, v_cache, k_exp, v_exp, B, H, D)
+    if out is None:
+        out = tuple(torch.empty((B, tokens, H, D), dtype=dtype, device=k_cache.device) for _ in range(2))
+    _check_same("kv_read_q8", k_cache, {"out[0]": (out[0], (B, tokens, H, D), dtype), "out[1]": (out[1], (B, tokens, H, D), dtype)})
+    if len(begin) < B:
+        raise ValueError("kv_read_q8: begin needs one entry per row")
+    if out[0].numel() == 0:
+        return out
+    views = [N.view(t) for t in (k_cache, v_cache)] + [_exp_view(k_exp), _exp_view(v_exp)] + [N.view(t) for t in out]
+    with _on_device(k_cache), _Logged("kv_read_q8", B * tokens * H * 2.0 * (D + 1 + D * out[0].element_size())):
+        rc = N.lib().sdv2_kv_read_q8(*[C.byref(x) for x in views], B, tokens, H, D, smax, N.i64_array(begin),
+                                     N.dtype_code(dtype), N.stream_ptr(k_cache.device))
+    N.check(rc, "sdv2_kv_read_q8")
+    return out
+
+
+def attn_kvcache_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_exp: torch.Tensor,
+                    v_exp: torch.Tensor, seq_lens: Sequence[int], *, out: Optional[torch.Tensor] = None,
+                    softmax_scale: Optional[float] = None) -> torch.Tensor:
+    """`attn_kvcache` over an 8-bit cache: softmax(q k^T scale) v over the values that cache[b, :seq_lens[b]] holds
+    (bf16 q and output).  seq_lens[b] may be 0: that row's output is 0."""
+    B, n_q, H, D = q.shape
+    if q.dtype != torch.bfloat16:
+        raise ValueError("the tensor-core attention kernel takes bf16")
+    smax = _check_q8("attn_kvcache_q8", q, k_cache, v_cache, k_exp, v_exp, B, H, D)
+    if out is None:
+        out = torch.empty((B, n_q, H, D), dtype=q.dtype, device=q.device)
+    _check_same("attn_kvcache_q8", q, {"out": (out, q.shape, q.dtype)})
+    if len(seq_lens) < B:
+        raise ValueError("attn_kvcache_q8: seq_lens needs one entry per row")
+    if q.numel() == 0 or smax == 0:
+        return out.zero_()
+    scale = softmax_scale if softmax_scale is not None else 1.0 / math.sqrt(D)
+    lens = N.i32_array(seq_lens)
+    views = [N.view(t) for t in (q, k_cache, v_cache)] + [_exp_view(k_exp), _exp_view(v_exp), N.view(out)]
+    with _on_device(q):
+        lib = N.lib()
+        scratch = _scratch(lib.sdv2_attn_q8_scratch_bytes(B, n_q, H, smax, lens), q.device)
+        args = [*[C.byref(x) for x in views], B, n_q, H, D, smax, lens, scale, *scratch[1:], workspace(q.device).data_ptr(),
+                N.stream_ptr(q.device)]
+        with _Logged("attn_kvcache_q8", 4.0 * n_q * D * H * float(sum(int(x) for x in seq_lens[:B]))):
+            rc = lib.sdv2_attn_kvcache_q8(*args)
+    N.check(rc, "sdv2_attn_kvcache_q8")
+    return out
+
+
+def _scratch(nbytes: int, device):
+    """(tensor to keep until the launch, pointer, bytes) of a call's own scratch.  It comes from PyTorch's allocator on
+    the launching stream (a graph's own pool while capturing), so calls on other streams and other recorded graphs never
+    share it."""
+    if nbytes == 0:
+        return None, None, 0
+    t = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    return t, t.data_ptr(), nbytes
+
+
+def attn_spans(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, begin: Optional[torch.Tensor], end: torch.Tensor, *,
+               out: Optional[torch.Tensor] = None, softmax_scale: Optional[float] = None) -> torch.Tensor:
+    """Attention in which query i of row b attends the keys begin[b, i] <= j < end[b, i] only: prompt lengths,
+    block-causal clips, clips packed into one row, windows.  q [B, N, H, 128], k / v [B, S, H, 128] bf16 (k / v may be
+    stride-0 expands over rows); begin (None: 0) and end int32 [B, N] on the device, any strides (an expanded [B, 1]
+    does for one span per row).  Spans are clipped to the keys there are; a query with an empty span gets 0.  K and V of
+    keys that no query attends may hold anything."""
+    B, n_q, H, D = q.shape
+    if q.dtype != torch.bfloat16:
+        raise ValueError("the tensor-core attention kernel takes bf16")
+    S = k.shape[1]
+    if out is None:
+        out = torch.empty((B, n_q, H, D), dtype=q.dtype, device=q.device)
+    wanted = {"k": (k, (B, S, H, D), q.dtype), "v": (v, (B, S, H, D), q.dtype), "out": (out, q.shape, q.dtype),
+              "end": (end, (B, n_q), torch.int32)}
+    if begin is not None:
+        wanted["begin"] = (begin, (B, n_q), torch.int32)
+    _check_same("attn_spans", q, wanted)
+    if q.numel() == 0 or S == 0:
+        return out.zero_()
+    scale = softmax_scale if softmax_scale is not None else 1.0 / math.sqrt(D)
+    views = [N.view(t) for t in (q, k, v, out)]
+    b_args = (None, 0, 0) if begin is None else (begin.data_ptr(), *begin.stride())
+    with _on_device(q):
+        lib = N.lib()
+        scratch = _scratch(lib.sdv2_attn_spans_scratch_bytes(B, n_q, H, S), q.device)
+        args = [*[C.byref(x) for x in views], B, n_q, H, D, S, *b_args, end.data_ptr(), *end.stride(), scale, *scratch[1:],
+                workspace(q.device).data_ptr(), N.stream_ptr(q.device)]
+        with _Logged("attn_spans"):
+            rc = lib.sdv2_attn_spans(*args)
+    N.check(rc, "sdv2_attn_spans")
     return out
 
 
