@@ -80,19 +80,20 @@ _SIGNATURES = {
     "sdv2_residual_layernorm": (C.c_int, [C.c_void_p] * 3 + [C.c_int64, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p,
                                                              C.c_int64, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int,
                                                              C.c_float, C.c_void_p]),
-    "sdv2_rope_kv_append_q8": (C.c_int, [C.POINTER(View)] * 8 + [C.c_int, C.c_int, C.c_int, C.c_int, C.c_int64,
+    # views of these four are passed as addresses: building View objects would cost a small call several microseconds
+    "sdv2_rope_kv_append_q8": (C.c_int, [C.c_void_p] * 8 + [C.c_int, C.c_int, C.c_int, C.c_int, C.c_int64,
                                                                   C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int,
                                                                   C.POINTER(C.c_int64), C.POINTER(C.c_int64),
                                                                   C.c_void_p, C.c_void_p, C.c_void_p,
                                                                   C.POINTER(C.c_int64), C.POINTER(C.c_int64),
                                                                   C.c_int, C.c_void_p, C.c_void_p]),
-    "sdv2_kv_read_q8": (C.c_int, [C.POINTER(View)] * 6 + [C.c_int, C.c_int, C.c_int, C.c_int, C.c_int64,
+    "sdv2_kv_read_q8": (C.c_int, [C.c_void_p] * 6 + [C.c_int, C.c_int, C.c_int, C.c_int, C.c_int64,
                                                           C.POINTER(C.c_int64), C.c_int, C.c_void_p]),
-    "sdv2_attn_kvcache_q8": (C.c_int, [C.POINTER(View)] * 6 + [C.c_int, C.c_int, C.c_int, C.c_int, C.c_int64,
+    "sdv2_attn_kvcache_q8": (C.c_int, [C.c_void_p] * 6 + [C.c_int, C.c_int, C.c_int, C.c_int, C.c_int64,
                                                                C.POINTER(C.c_int32), C.c_float, C.c_void_p,
                                                                C.c_size_t, C.c_void_p, C.c_void_p]),
     "sdv2_attn_q8_scratch_bytes": (C.c_size_t, [C.c_int, C.c_int, C.c_int, C.c_int64, C.POINTER(C.c_int32)]),
-    "sdv2_attn_spans": (C.c_int, [C.POINTER(View)] * 4 + [C.c_int, C.c_int, C.c_int, C.c_int, C.c_int64,
+    "sdv2_attn_spans": (C.c_int, [C.c_void_p] * 4 + [C.c_int, C.c_int, C.c_int, C.c_int, C.c_int64,
                                                           C.c_void_p, C.c_int64, C.c_int64, C.c_void_p, C.c_int64,
                                                           C.c_int64, C.c_float, C.c_void_p, C.c_size_t, C.c_void_p,
                                                           C.c_void_p]),

@@ -521,6 +521,7 @@ int sdv2_kv_read_q8(const sdv2_view* k_cache, const sdv2_view* v_cache, const sd
   for (int b = 0; b < rows; ++b) {
     if (begin[b] < 0 || begin[b] > cache_tokens - tokens) return SDV2_ERR_INVALID_ARG;
     p.begin[b] = begin[b];
+    p.count[b] = tokens;
   }
   p.k = *k_cache; p.v = *v_cache; p.k_exp = *k_exp; p.v_exp = *v_exp; p.k_out = *k_out; p.v_out = *v_out;
   p.rows = rows; p.tokens = tokens; p.heads = heads; p.dtype = dtype;
@@ -541,14 +542,6 @@ static int fill_attn_x(sdv2::AttnXParams& p, int rows, int q_tokens, int heads, 
   return SDV2_OK;
 }
 
-static int plan_of(sdv2::AttnXParams& p, bool q8, int* slots) {
-  sdv2::DeviceInfo di;
-  const cudaError_t e = sdv2::device_info(&di);
-  if (e != cudaSuccess) return cuda_fail(e);
-  *slots = q8 ? sdv2::plan_q8(p, di.sms) : sdv2::plan_spans(p, di.sms);
-  return *slots < 0 ? SDV2_ERR_UNSUPPORTED_SHAPE : SDV2_OK;
-}
-
 static int fill_lens(sdv2::AttnXParams& p, const int32_t* seq_lens) {
   if (seq_lens == nullptr) return SDV2_ERR_INVALID_ARG;
   for (int b = 0; b < p.rows; ++b) {
@@ -558,8 +551,8 @@ static int fill_lens(sdv2::AttnXParams& p, const int32_t* seq_lens) {
   return SDV2_OK;
 }
 
-static int attn_x_common(sdv2::AttnXParams& p, bool q8, const sdv2_view* q, const sdv2_view* out, int head_dim,
-                         float softmax_scale, void* scratch, size_t scratch_bytes, int* status) {
+static int fill_q_out(sdv2::AttnXParams& p, const sdv2_view* q, const sdv2_view* out, int head_dim, float softmax_scale,
+                      int* status) {
   if (head_dim != 128) return SDV2_ERR_UNSUPPORTED_SHAPE;
   int rc;
   if ((rc = check_view(q, 2, false)) != SDV2_OK || (rc = check_view(out, 2, false)) != SDV2_OK) return rc;
@@ -570,50 +563,140 @@ static int attn_x_common(sdv2::AttnXParams& p, bool q8, const sdv2_view* q, cons
   p.out_stride_head = out->stride_head;
   p.scale_log2 = softmax_scale * 1.4426950408889634f;
   p.status = status;
-  int slots = 0;
-  if ((rc = plan_of(p, q8, &slots)) != SDV2_OK) return rc;
-  if (slots > 0) {
-    if (scratch == nullptr || scratch_bytes < slots * sdv2::kAttnXPartFloats * sizeof(float)) return SDV2_ERR_WORKSPACE;
-    if (!aligned16(scratch)) return SDV2_ERR_MISALIGNED;
-    p.part_o = static_cast<float*>(scratch);
-    p.part_meta = p.part_o + static_cast<size_t>(slots) * 2 * 128 * 128;
+  return SDV2_OK;
+}
+
+static size_t partial_bytes(int slots) { return slots * sdv2::kAttnXPartFloats * sizeof(float); }
+
+static void set_partials(sdv2::AttnXParams& p, void* scratch, int slots) {
+  p.part_o = slots > 0 ? static_cast<float*>(scratch) : nullptr;
+  p.part_meta = slots > 0 ? p.part_o + static_cast<size_t>(slots) * 2 * 128 * 128 : nullptr;
+}
+
+// How attention over the 8-bit cache runs.  Expanding K/V inside the attention kernel reads each byte once per pair of
+// query tiles and takes shared-memory bandwidth from the tensor cores (about 4400 cycles a key tile against 3250);
+// expanding them to bf16 scratch first costs 6 bytes of HBM traffic a value once, 3900 cycles' share of a key tile.  So
+// from four pairs of query tiles on (more than 768 queries) the cache is expanded first, a group of heads at a time so
+// that the scratch stays near 1 GiB.
+struct Q8Run {
+  sdv2::AttnXParams p;  // of one head group when expanding first
+  int group, longest;
+  int slots;        // partial-result slots of the group size that needs the most
+  size_t expanded;  // bytes of K, and of V, for one head group
+};
+
+static int fill_q8(Q8Run& r, int rows, int q_tokens, int heads, int64_t cache_tokens, const int32_t* seq_lens) {
+  constexpr int kExpandFirstPairTiles = 4;
+  constexpr int64_t kGroupBytes = 512ll << 20;
+  int rc;
+  if ((rc = fill_attn_x(r.p, rows, q_tokens, heads, cache_tokens)) != SDV2_OK || (rc = fill_lens(r.p, seq_lens)) != SDV2_OK)
+    return rc;
+  r.group = heads;
+  r.longest = 0;
+  r.expanded = 0;
+  for (int b = 0; b < rows; ++b) r.longest = r.longest > seq_lens[b] ? r.longest : seq_lens[b];
+  if (r.p.pair_tiles >= kExpandFirstPairTiles && r.longest > 0) {
+    const int64_t per_head = static_cast<int64_t>(rows) * r.longest * 256;
+    const int64_t fit = kGroupBytes / per_head;
+    r.group = fit >= heads ? heads : (fit < 1 ? 1 : static_cast<int>(fit));
+    r.group = (heads + (heads + r.group - 1) / r.group - 1) / ((heads + r.group - 1) / r.group);  // groups of equal size
+    r.expanded = static_cast<size_t>(per_head) * r.group;
   }
   return SDV2_OK;
 }
 
+static int plan_q8(Q8Run& r, int heads) {
+  sdv2::DeviceInfo di;
+  const cudaError_t e = sdv2::device_info(&di);
+  if (e != cudaSuccess) return cuda_fail(e);
+  int last = 0;
+  if (heads % r.group != 0) {  // a smaller last group
+    r.p.heads = heads % r.group;
+    last = sdv2::plan_lens(r.p, di.sms);
+  }
+  r.p.heads = r.group;
+  r.slots = sdv2::plan_lens(r.p, di.sms);
+  if (r.slots < 0 || last < 0) return SDV2_ERR_UNSUPPORTED_SHAPE;
+  if (last > r.slots) r.slots = last;
+  return SDV2_OK;
+}
+
 size_t sdv2_attn_q8_scratch_bytes(int rows, int q_tokens, int heads, int64_t cache_tokens, const int32_t* seq_lens) {
-  sdv2::AttnXParams p;
-  int slots = 0;
-  if (fill_attn_x(p, rows, q_tokens, heads, cache_tokens) != SDV2_OK || fill_lens(p, seq_lens) != SDV2_OK ||
-      plan_of(p, true, &slots) != SDV2_OK)
-    return 0;
-  return slots * sdv2::kAttnXPartFloats * sizeof(float);
+  Q8Run r;
+  if (fill_q8(r, rows, q_tokens, heads, cache_tokens, seq_lens) != SDV2_OK || plan_q8(r, heads) != SDV2_OK) return 0;
+  return 2 * r.expanded + partial_bytes(r.slots);
 }
 
 int sdv2_attn_kvcache_q8(const sdv2_view* q, const sdv2_view* k_cache, const sdv2_view* v_cache, const sdv2_view* k_exp,
                          const sdv2_view* v_exp, const sdv2_view* out, int rows, int q_tokens, int heads, int head_dim,
                          int64_t cache_tokens, const int32_t* seq_lens, float softmax_scale, void* scratch_dev,
                          size_t scratch_bytes, int* status_dev, void* stream) {
-  sdv2::AttnXParams p;
+  Q8Run r;
   int rc;
-  if ((rc = fill_attn_x(p, rows, q_tokens, heads, cache_tokens)) != SDV2_OK) return rc;
-  if ((rc = fill_lens(p, seq_lens)) != SDV2_OK) return rc;
   if ((rc = check_view(k_cache, 1, true)) != SDV2_OK || (rc = check_view(v_cache, 1, true)) != SDV2_OK) return rc;
   if ((rc = check_exps(k_exp, true)) != SDV2_OK || (rc = check_exps(v_exp, true)) != SDV2_OK) return rc;
-  if ((rc = attn_x_common(p, true, q, out, head_dim, softmax_scale, scratch_dev, scratch_bytes, status_dev)) != SDV2_OK)
-    return rc;
-  p.k = *k_cache; p.v = *v_cache; p.k_exp = *k_exp; p.v_exp = *v_exp;
-  CUtensorMap tm_q;
-  if ((rc = make_tile_map(&tm_q, q, rows, q_tokens, heads)) != SDV2_OK) return rc;
-  const cudaError_t e = sdv2::launch_attn_q8(tm_q, p, static_cast<cudaStream_t>(stream));
-  return e == cudaSuccess ? SDV2_OK : cuda_fail(e);
+  if ((rc = fill_q8(r, rows, q_tokens, heads, cache_tokens, seq_lens)) != SDV2_OK) return rc;
+  if ((rc = fill_q_out(r.p, q, out, head_dim, softmax_scale, status_dev)) != SDV2_OK) return rc;
+  if ((rc = plan_q8(r, heads)) != SDV2_OK) return rc;
+  const size_t need = 2 * r.expanded + partial_bytes(r.slots);
+  if (need > 0 && (scratch_dev == nullptr || scratch_bytes < need)) return SDV2_ERR_WORKSPACE;
+  if (!aligned16(scratch_dev)) return SDV2_ERR_MISALIGNED;
+  char* scratch = static_cast<char*>(scratch_dev);
+  set_partials(r.p, scratch + 2 * r.expanded, r.slots);
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  CUtensorMap tm_q, tm_k, tm_v;
+  cudaError_t e = cudaSuccess;
+  if (r.expanded == 0) {
+    r.p.k = *k_cache; r.p.v = *v_cache; r.p.k_exp = *k_exp; r.p.v_exp = *v_exp;
+    if ((rc = make_tile_map(&tm_q, q, rows, q_tokens, heads)) != SDV2_OK) return rc;
+    e = sdv2::launch_attn_q8_expand(tm_q, r.p, s);
+    return e == cudaSuccess ? SDV2_OK : cuda_fail(e);
+  }
+  for (int h0 = 0; h0 < heads; h0 += r.group) {
+    const int n = heads - h0 < r.group ? heads - h0 : r.group;
+    const int64_t tok = static_cast<int64_t>(n) * 128;
+    const sdv2_view kx = {scratch, r.longest * tok, tok, 128}, vx = {scratch + r.expanded, r.longest * tok, tok, 128};
+    auto from = [&](const sdv2_view* v, int esize) {
+      sdv2_view w = *v;
+      w.ptr = static_cast<char*>(v->ptr) + h0 * v->stride_head * esize;
+      return w;
+    };
+    sdv2::Q8ReadParams rp;
+    memset(&rp, 0, sizeof(rp));
+    rp.k = from(k_cache, 1); rp.v = from(v_cache, 1); rp.k_exp = from(k_exp, 1); rp.v_exp = from(v_exp, 1);
+    rp.k_out = kx; rp.v_out = vx;
+    rp.rows = rows; rp.tokens = r.longest; rp.heads = n; rp.dtype = SDV2_DTYPE_BF16;
+    for (int b = 0; b < rows; ++b) rp.count[b] = seq_lens[b];
+    const sdv2_view qg = from(q, 2), og = from(out, 2);
+    r.p.out = og.ptr;
+    if (n != r.p.heads) {  // a smaller last group is cut up anew
+      sdv2::DeviceInfo di;
+      if ((e = sdv2::device_info(&di)) != cudaSuccess) return cuda_fail(e);
+      r.p.heads = n;
+      if (sdv2::plan_lens(r.p, di.sms) < 0) return SDV2_ERR_UNSUPPORTED_SHAPE;
+    }
+    if ((rc = make_tile_map(&tm_q, &qg, rows, q_tokens, n)) != SDV2_OK) return rc;
+    if ((rc = make_tile_map(&tm_k, &kx, rows, r.longest, n)) != SDV2_OK) return rc;
+    if ((rc = make_tile_map(&tm_v, &vx, rows, r.longest, n)) != SDV2_OK) return rc;
+    if ((e = sdv2::launch_kv_read_q8(rp, s)) != cudaSuccess) return cuda_fail(e);
+    if ((e = sdv2::launch_attn_lens(tm_q, tm_k, tm_v, r.p, s)) != cudaSuccess) return cuda_fail(e);
+  }
+  return SDV2_OK;
+}
+
+static int plan_spans(sdv2::AttnXParams& p, int* slots) {
+  sdv2::DeviceInfo di;
+  const cudaError_t e = sdv2::device_info(&di);
+  if (e != cudaSuccess) return cuda_fail(e);
+  *slots = sdv2::plan_spans(p, di.sms);
+  return *slots < 0 ? SDV2_ERR_UNSUPPORTED_SHAPE : SDV2_OK;
 }
 
 size_t sdv2_attn_spans_scratch_bytes(int rows, int q_tokens, int heads, int64_t kv_tokens) {
   sdv2::AttnXParams p;
   int slots = 0;
-  if (fill_attn_x(p, rows, q_tokens, heads, kv_tokens) != SDV2_OK || plan_of(p, false, &slots) != SDV2_OK) return 0;
-  return slots * sdv2::kAttnXPartFloats * sizeof(float);
+  if (fill_attn_x(p, rows, q_tokens, heads, kv_tokens) != SDV2_OK || plan_spans(p, &slots) != SDV2_OK) return 0;
+  return partial_bytes(slots);
 }
 
 int sdv2_attn_spans(const sdv2_view* q, const sdv2_view* k, const sdv2_view* v, const sdv2_view* out, int rows,
@@ -629,8 +712,12 @@ int sdv2_attn_spans(const sdv2_view* q, const sdv2_view* k, const sdv2_view* v, 
   if (begin_stride_row < 0 || begin_stride_tok < 0 || end_stride_row < 0 || end_stride_tok < 0) return SDV2_ERR_INVALID_ARG;
   if ((rc = check_view(k, 2, true)) != SDV2_OK || (rc = check_view(v, 2, true)) != SDV2_OK) return rc;
   if ((k->stride_row == 0) != (v->stride_row == 0)) return SDV2_ERR_INVALID_ARG;
-  if ((rc = attn_x_common(p, false, q, out, head_dim, softmax_scale, scratch_dev, scratch_bytes, status_dev)) != SDV2_OK)
-    return rc;
+  if ((rc = fill_q_out(p, q, out, head_dim, softmax_scale, status_dev)) != SDV2_OK) return rc;
+  int slots = 0;
+  if ((rc = plan_spans(p, &slots)) != SDV2_OK) return rc;
+  if (slots > 0 && (scratch_dev == nullptr || scratch_bytes < partial_bytes(slots))) return SDV2_ERR_WORKSPACE;
+  if (!aligned16(scratch_dev)) return SDV2_ERR_MISALIGNED;
+  set_partials(p, scratch_dev, slots);
   p.kv_row_broadcast = k->stride_row == 0 ? 1 : 0;
   p.begin = begin_dev;
   p.end = end_dev;

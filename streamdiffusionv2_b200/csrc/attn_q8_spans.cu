@@ -4,7 +4,7 @@
 // S = Q K^T and O += P V (tcgen05, fp32 in TMEM), a softmax warpgroup per query tile, K/V through a ring of five
 // 32 KB tiles handed over as pairs (V_j, K_j+1), lazy rescaling of O.  What differs:
 //
-// kQ8.  K/V tiles are not copied by TMA: three warps load the cache's bytes into registers one tile ahead, expand them
+// kQ8.  K/V tiles are not copied by TMA: four warps load the cache's bytes into registers one tile ahead, expand them
 //   to bf16 and store them in the layout the tensor cores read.  A tile of K carries the largest exponent E of its
 //   tokens: it holds m * 2^(e-E-6), and 2^(E+6) joins the softmax scale of that tile, one multiplication per tile.  V
 //   tiles use R, the largest exponent of V so far, the same way; when R grows O is rescaled, as for a grown maximum.
@@ -33,8 +33,33 @@ namespace attnx {
 using namespace attn;
 
 constexpr int kRing = 5;
-constexpr int kThreads = 384;
-constexpr int kExpandWarps = 3;
+constexpr int kExpandWarps = 4;
+// Warpgroups: 0 = the issuing warp (and the TMA warp of the span kernel), then with kQ8 one that expands the cache's
+// bytes, then one softmax warpgroup per query tile.  Registers move from the former to the latter: 2 x 176 + 48 + 112 of
+// 4 x 128 a thread at launch, 2 x 200 + 104 of 3 x 168 without the expand warpgroup.
+enum Mode {
+  kModeSpans,   // K/V tensors by TMA, a span of keys per query
+  kModeExpand,  // 8-bit cache, expanded in the kernel
+  kModeLens,    // K/V tensors by TMA, one length per row: the 8-bit cache after kv_read_q8_kernel
+};
+
+template <bool kQ8>
+struct Roles {
+  static constexpr int kSoftmaxWarp0 = kQ8 ? 8 : 4;
+  static constexpr int kThreads = (kSoftmaxWarp0 + 8) * 32;
+  static constexpr int kRegsIssue = kQ8 ? 48 : 104, kRegsExpand = 112, kRegsSoftmax = kQ8 ? 176 : 200;
+  static constexpr int kRegsLaunch = kQ8 ? 128 : 168;
+  static_assert((kQ8 ? kRegsIssue + kRegsExpand : kRegsIssue) + 2 * kRegsSoftmax <= kRegsLaunch * kThreads / 128,
+                "the warpgroups' shares add up to more than the launch provides");
+};
+template <int kRegs>
+__device__ __forceinline__ void regs_dec() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs));
+}
+template <int kRegs>
+__device__ __forceinline__ void regs_inc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs));
+}
 constexpr uint32_t kSmemQ = 0;
 constexpr uint32_t kSmemKV = 2 * kTileBytes;
 constexpr uint32_t kSmemBar = kSmemKV + kRing * kTileBytes;
@@ -66,59 +91,66 @@ __device__ __forceinline__ float exp2_int(int e) {  // 2^e, e clamped to fp32's 
 }
 
 // ------------------------------------------------------------------ expanding the 8-bit cache (kQ8)
-// A tile is 32 groups of four tokens; expand warp w takes groups w, w + 3, ...  In a group a token has eight lanes of
-// 16 bytes each.
-constexpr int kGroups = (32 + kExpandWarps - 1) / kExpandWarps;
+// A tile is 8 steps x 4 warps of four tokens.  A lane has 16 bytes of one token: in every eight lanes, 64 bytes of an
+// even token and of the odd one after it, whose swizzled chunks never share a bank.
+constexpr int kSteps = 8;
 
 struct TileBytes {
-  uint4 raw[kGroups];
+  uint4 raw[kSteps];
+};
+__device__ __forceinline__ int lane_token(int lane) { return ((lane >> 4) << 1) | ((lane >> 2) & 1); }  // 0..3
+__device__ __forceinline__ int lane_byte(int lane) { return ((lane >> 3) & 1) * 64 + (lane & 3) * 16; }
+
+// Four of the 128 exponents of a tile: tokens lane, lane + 32, ...  Tokens past the end get the smallest exponent.
+struct TileExps {
+  int e[4];
+  __device__ __forceinline__ void load(const int8_t* base, int64_t stride_tok, int tok0, int seq_len, int lane) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int t = tok0 + i * 32 + lane;
+      e[i] = t < seq_len ? base[t * stride_tok] : q8::kMinExp;
+    }
+  }
+  // largest of the tile's exponents; vectors that are not finite carry -128 and leave it to the others
+  __device__ __forceinline__ int top() const {
+    return __reduce_max_sync(0xffffffffu, max(max(max(e[0], e[1]), max(e[2], e[3])), q8::kMinExp));
+  }
+  __device__ __forceinline__ uint32_t packed() const {
+    return __byte_perm(__byte_perm(e[0], e[1], 0x0040), __byte_perm(e[2], e[3], 0x0040), 0x5410);
+  }
 };
 
-// The lane's share of the 128 exponents of a tile: tokens lane, lane + 32, ... as four bytes.  Tokens past the end get
-// the smallest exponent.
-__device__ __forceinline__ uint32_t load_exps(const int8_t* base, int64_t stride_tok, int tok0, int seq_len, int lane) {
-  uint32_t packed = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int t = tok0 + i * 32 + lane;
-    const int e = t < seq_len ? base[static_cast<int64_t>(t) * stride_tok] : q8::kMinExp;
-    packed |= (static_cast<uint32_t>(e) & 0xFFu) << (8 * i);
-  }
-  return packed;
+// 16 bytes that no one reads again on this SM: not kept in L1, which shared memory leaves little of
+__device__ __forceinline__ uint4 ld_stream(const uint8_t* p) {
+  uint4 v;
+  asm("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
 }
 
-__device__ __forceinline__ int max_exp(uint32_t packed) {
-  int e = q8::kMinExp;  // vectors that are not finite carry -128 and leave it to the others
+// `base`: this lane's bytes of token 0; `tok`: this lane's token of step 0.
+__device__ __forceinline__ void load_bytes(TileBytes& t, const uint8_t* base, int64_t stride_tok, int tok, int seq_len) {
+  const uint8_t* src = base + tok * stride_tok;
+  const int64_t step = 16 * stride_tok;
+  if (__all_sync(0xffffffffu, tok + 16 * (kSteps - 1) < seq_len)) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) e = max(e, static_cast<int>(static_cast<int8_t>(packed >> (8 * i))));
-  return __reduce_max_sync(0xffffffffu, e);
-}
-
-__device__ __forceinline__ void load_bytes(TileBytes& t, const uint8_t* base, int64_t stride_tok, int tok0, int seq_len,
-                                           int w, int lane) {
+    for (int i = 0; i < kSteps; ++i) t.raw[i] = ld_stream(src + i * step);
+  } else {
 #pragma unroll
-  for (int i = 0; i < kGroups; ++i) {
-    const int g = i * kExpandWarps + w;
-    const int tok = tok0 + g * 4 + (lane >> 3);
-    t.raw[i] = make_uint4(0u, 0u, 0u, 0u);
-    if (g < 32 && tok < seq_len)
-      t.raw[i] = __ldg(reinterpret_cast<const uint4*>(base + static_cast<int64_t>(tok) * stride_tok) + (lane & 7));
+    for (int i = 0; i < kSteps; ++i)
+      t.raw[i] = tok + 16 * i < seq_len ? ld_stream(src + i * step) : make_uint4(0u, 0u, 0u, 0u);
   }
 }
 
 // Store the tile as bf16 m * 2^(e - ref - 6) in the 128-byte-swizzled layout of two 64-column halves.
-__device__ __forceinline__ void expand_tile(const TileBytes& t, uint32_t exps, int ref, uint8_t* tile, int w, int lane) {
-  const int c = lane & 7;
-  uint8_t* half = tile + (c >> 2) * kHalfTile;
-  const int ch = (2 * c) & 7;
-  const bool swap = c >= 4;  // the two halves store their chunks in opposite order: no bank is hit twice
+__device__ __forceinline__ void expand_tile(const TileBytes& t, uint32_t exps, int ref, uint32_t tile, int w, int lane) {
+  const int sub = w * 4 + lane_token(lane);  // token of step i: 16 i + sub
+  // the four exponents of the tokens sub + 32 k and of sub + 16 + 32 k
+  const uint32_t even = __shfl_sync(0xffffffffu, exps, sub), odd = __shfl_sync(0xffffffffu, exps, sub + 16);
+  const uint32_t row = tile + ((lane >> 3) & 1) * kHalfTile + sub * 128;
+  const uint32_t first = row + ((((lane & 3) * 2) ^ (sub & 7)) << 4), second = row + ((((lane & 3) * 2 + 1) ^ (sub & 7)) << 4);
 #pragma unroll
-  for (int i = 0; i < kGroups; ++i) {
-    const int g = i * kExpandWarps + w;
-    if (g >= 32) break;
-    const int tl = g * 4 + (lane >> 3);
-    const uint32_t ev = __shfl_sync(0xffffffffu, exps, tl & 31) >> (8 * (tl >> 5));
-    const int e = static_cast<int8_t>(ev);
+  for (int i = 0; i < kSteps; ++i) {
+    const int e = static_cast<int8_t>(((i & 1) ? odd : even) >> (8 * (i >> 1)));
     // 2^(127 + e - ref) times the subnormal m * 2^-133; e <= ref, so the multiplier is a normal bf16 number
     const uint32_t s2 = e == q8::kNotFinite ? 0x7FC07FC0u : static_cast<uint32_t>(254 + e - ref) * 0x00800080u;
     const uint32_t in[4] = {t.raw[i].x, t.raw[i].y, t.raw[i].z, t.raw[i].w};
@@ -129,11 +161,8 @@ __device__ __forceinline__ void expand_tile(const TileBytes& t, uint32_t exps, i
       o[2 * k] = q8::mul_bf16x2(o[2 * k], s2);
       o[2 * k + 1] = q8::mul_bf16x2(o[2 * k + 1], s2);
     }
-    const uint4 first = make_uint4(o[0], o[1], o[2], o[3]), second = make_uint4(o[4], o[5], o[6], o[7]);
-    uint8_t* row = half + tl * 128;
-    const int x = tl & 7;
-    *reinterpret_cast<uint4*>(row + (((swap ? ch + 1 : ch) ^ x) << 4)) = swap ? second : first;
-    *reinterpret_cast<uint4*>(row + (((swap ? ch : ch + 1) ^ x) << 4)) = swap ? first : second;
+    st_shared_v4(first + i * 2048, o[0], o[1], o[2], o[3]);
+    st_shared_v4(second + i * 2048, o[4], o[5], o[6], o[7]);
   }
 }
 
@@ -142,14 +171,14 @@ struct Item {
   int b, h, q0, part, parts, slot;  // part < 0: the whole key range, written to the output directly
 };
 
-template <bool kQ8>
+template <bool kSpans>
 __device__ __forceinline__ Item find_item(const AttnXParams& p, int i) {
   Item it;
   int pt, hb;
   it.part = -1;
   it.parts = 1;
   it.slot = 0;
-  if (kQ8) {
+  if (!kSpans) {
     int tile = i, r = 0;
     if (i >= p.n_full) {
       const int k = i - p.n_full;
@@ -167,10 +196,13 @@ __device__ __forceinline__ Item find_item(const AttnXParams& p, int i) {
     it.b = p.order[hb / p.heads];
   } else {
     // late query tiles first: with masks that grow along the sequence they are the long ones
-    const int tile = i / p.split;
-    if (p.split > 1) it.part = i % p.split;
-    it.parts = p.split;
-    it.slot = i;
+    int tile = i;
+    if (i >= p.n_full) {
+      it.slot = i - p.n_full;
+      tile = p.n_full + it.slot / p.split;
+      it.parts = p.split;
+      if (p.split > 1) it.part = it.slot % p.split;
+    }
     const int per = p.heads * p.rows;
     pt = p.pair_tiles - 1 - tile / per;
     hb = tile % per;
@@ -181,10 +213,11 @@ __device__ __forceinline__ Item find_item(const AttnXParams& p, int i) {
   return it;
 }
 
-template <bool kQ8>
-__global__ void __launch_bounds__(kThreads, 1)
+template <int kMode>
+__global__ void __launch_bounds__(Roles<kMode == kModeExpand>::kThreads, 1)
 attn_x_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
               const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ AttnXParams p) {
+  constexpr bool kQ8 = kMode == kModeExpand, kSpans = kMode == kModeSpans;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
@@ -196,7 +229,7 @@ attn_x_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
   const int lane = threadIdx.x & 31;
-  const Item item = find_item<kQ8>(p, blockIdx.x);
+  const Item item = find_item<kSpans>(p, blockIdx.x);
   const int b = item.b, h = item.h, q0 = item.q0;
   const bool two_tiles = q0 + kBM < p.q_tokens;
   const int bk = p.kv_row_broadcast ? 0 : b;
@@ -230,8 +263,9 @@ attn_x_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
   }
   // this thread's query row (softmax warps) and its span, clipped to the keys there are
   int span_lo = 0, span_hi = 0;
-  const int my_row = q0 + (warp - 4) * 32 + lane;  // warps 4..11 are rows 0..255 of the tile pair
-  if (!kQ8 && warp >= 4 && my_row < p.q_tokens) {
+  constexpr int kSoftmaxWarp0 = Roles<kQ8>::kSoftmaxWarp0;
+  const int my_row = q0 + (warp - kSoftmaxWarp0) * 32 + lane;  // eight warps for the 256 rows of the tile pair
+  if (kSpans && warp >= kSoftmaxWarp0 && my_row < p.q_tokens) {
     const int64_t at = b * p.end_stride_row + static_cast<int64_t>(my_row) * p.end_stride_tok;
     span_hi = min(p.end[at], p.kv_tokens);
     if (p.begin != nullptr)
@@ -241,13 +275,13 @@ attn_x_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (!kQ8) {
+  if (kSpans) {
     const bool some = span_hi > span_lo;
     const int lo = __reduce_min_sync(0xffffffffu, some ? span_lo : 0x7FFFFFFF);
     const int hi = __reduce_max_sync(0xffffffffu, some ? span_hi : 0);
     const int flo = __reduce_max_sync(0xffffffffu, some ? span_lo : 0);
     const int fhi = __reduce_min_sync(0xffffffffu, some ? span_hi : 0x7FFFFFFF);
-    if (warp >= 4 && lane == 0) {
+    if (warp >= kSoftmaxWarp0 && lane == 0) {
       atomicMin(const_cast<int*>(words + kWordLo), lo);
       atomicMax(const_cast<int*>(words + kWordHi), hi);
       atomicMax(const_cast<int*>(words + kWordFullLo), flo);
@@ -257,8 +291,8 @@ attn_x_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
   }
   const uint32_t tmem = static_cast<uint32_t>(words[kWordTmem]);
   // the keys that some row attends, the key tiles they lie in, and this item's share of those
-  const int key_lo = kQ8 ? 0 : words[kWordLo], key_hi = kQ8 ? p.seq_lens[b] : words[kWordHi];
-  const int tile_lo = kQ8 ? 0 : (key_lo < key_hi ? key_lo / kBN : 0);
+  const int key_lo = kSpans ? words[kWordLo] : 0, key_hi = kSpans ? words[kWordHi] : p.seq_lens[b];
+  const int tile_lo = kSpans && key_lo < key_hi ? key_lo / kBN : 0;
   const int n_kv_all = key_lo < key_hi ? (key_hi + kBN - 1) / kBN - tile_lo : 0;
   const int j0 = tile_lo + (item.part < 0 ? 0 : static_cast<int>(static_cast<int64_t>(item.part) * n_kv_all / item.parts));
   const int j1 = tile_lo + (item.part < 0 ? n_kv_all
@@ -267,6 +301,7 @@ attn_x_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
 
   auto slot_off = [&](int it) { return kSmemKV + (it % kRing) * kTileBytes; };
 
+  if (warp < 4) regs_dec<Roles<kQ8>::kRegsIssue>();
   if (warp == 0) {
     // ------------------------------------------------------------------ MMA issuer
     if (lane == 0 && n_kv > 0) {
@@ -293,18 +328,24 @@ attn_x_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
       for (int j = 0; j < n_kv && ok; ++j) {
         const bool more = j + 1 < n_kv;
         const uint32_t sv = base + kSmemKV + slot_v * kTileBytes, sk = base + kSmemKV + slot_k * kTileBytes;
-        for (int s = 0; s < n_stage && ok; ++s) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          if (s >= n_stage || !ok) break;
+          // opaque to the compiler: descriptors are rebuilt from one address per tile instead of being kept, hoisted out
+          // of the loop, in registers that this warp does not have (spilled, they cost 300 cycles an MMA)
+          uint32_t q_tile = sq[s], s_col = tS[s], o_col = tO[s];
+          asm volatile("" : "+r"(q_tile), "+r"(s_col), "+r"(o_col));
           ok = mbar_wait(bar(kBarPHalf + s), j & 1, abort_flag, p.status, WAIT_P_FULL);
           if (ok && s == 0) ok = mbar_wait(bar(kBarPairFull + pair_bar), pair_par, abort_flag, p.status, WAIT_KV_FULL);
           if (!ok) break;
           tc_fence_after();
-          issue_pv(tO[s], tS[s], sv, j > 0, 0, 4);
+          issue_pv(o_col, s_col, sv, j > 0, 0, 4);
           ok = mbar_wait(bar(kBarPFull + s), j & 1, abort_flag, p.status, WAIT_P_FULL);
           if (!ok) break;
           tc_fence_after();
-          issue_pv(tO[s], tS[s], sv, true, 4, 8);
+          issue_pv(o_col, s_col, sv, true, 4, 8);
           if (more) {
-            issue_qk(tS[s], sq[s], sk);
+            issue_qk(s_col, q_tile, sk);
             umma_commit(bar(kBarSFull + s));
           } else {
             umma_commit(bar(kBarOFull + s));
@@ -319,32 +360,34 @@ attn_x_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
         }
       }
     }
-  } else if (warp < 4) {
-    if (kQ8) {
+  } else if (warp < kSoftmaxWarp0) {
+    if (kQ8 && warp >= 4) {
       // ---------------------------------------------------------------- expand warps
-      const int w = warp - 1;
-      const uint8_t* kb = static_cast<const uint8_t*>(p.k.ptr) + bk * p.k.stride_row + h * p.k.stride_head;
-      const uint8_t* vb = static_cast<const uint8_t*>(p.v.ptr) + bk * p.v.stride_row + h * p.v.stride_head;
+      regs_dec<Roles<kQ8>::kRegsExpand>();
+      const int w = warp - 4;
+      const int tok = j0 * kBN + w * 4 + lane_token(lane);
+      const uint8_t* kb = static_cast<const uint8_t*>(p.k.ptr) + bk * p.k.stride_row + h * p.k.stride_head + lane_byte(lane);
+      const uint8_t* vb = static_cast<const uint8_t*>(p.v.ptr) + bk * p.v.stride_row + h * p.v.stride_head + lane_byte(lane);
       const int8_t* keb = static_cast<const int8_t*>(p.k_exp.ptr) + bk * p.k_exp.stride_row + h * p.k_exp.stride_head;
       const int8_t* veb = static_cast<const int8_t*>(p.v_exp.ptr) + bk * p.v_exp.stride_row + h * p.v_exp.stride_head;
       TileBytes rk, rv;
-      uint32_t ek = 0, ev = 0, ev_next = 0;
+      TileExps ek, ev;
+      uint32_t ev_now = 0;
       int ref_v = q8::kMinExp, ref_next = q8::kMinExp;
       // K of a tile together with the exponents of its V, whose running maximum is published with K
       auto load_k = [&](int g) {
-        const int tok0 = (j0 + g) * kBN;
-        ek = load_exps(keb, p.k_exp.stride_tok, tok0, key_hi, lane);
-        ev_next = load_exps(veb, p.v_exp.stride_tok, tok0, key_hi, lane);
-        load_bytes(rk, kb, p.k.stride_tok, tok0, key_hi, w, lane);
+        ek.load(keb, p.k_exp.stride_tok, (j0 + g) * kBN, key_hi, lane);
+        ev.load(veb, p.v_exp.stride_tok, (j0 + g) * kBN, key_hi, lane);
+        load_bytes(rk, kb, p.k.stride_tok, tok + g * kBN, key_hi);
       };
       auto expand_k = [&](int g, int it) {
-        const int ref = max_exp(ek);
-        ref_next = max(ref_next, max_exp(ev_next));
+        const int ref = ek.top();
+        ref_next = max(ref_next, ev.top());
         if (w == 0 && lane == 0) {
           words[kWordExpK + (g & 3)] = ref;
           words[kWordExpV + (g & 3)] = ref_next;
         }
-        expand_tile(rk, ek, ref, gbase + slot_off(it), w, lane);
+        expand_tile(rk, ek.packed(), ref, base + slot_off(it), w, lane);
       };
       auto arrive = [&](int i) {
         fence_proxy_async_smem();
@@ -353,13 +396,13 @@ attn_x_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
       };
       if (n_kv > 0) {
         load_k(0);
-        load_bytes(rv, vb, p.v.stride_tok, j0 * kBN, key_hi, w, lane);
+        load_bytes(rv, vb, p.v.stride_tok, tok, key_hi);
         expand_k(0, 0);
         arrive(kBarK0Full);
       }
       for (int g = 0; g < n_kv; ++g) {  // pair g = items 2g+1 (V_g) and 2g+2 (K_{g+1})
         const bool more = g + 1 < n_kv;
-        ev = ev_next;
+        ev_now = ev.packed();
         ref_v = ref_next;
         if (more) load_k(g + 1);
         // the slots of pair g held K_{g-2} and V_{g-2}: free once step g-2 of the issuer has completed
@@ -368,14 +411,14 @@ attn_x_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
                               WAIT_KV_EMPTY);
           if (!__all_sync(0xffffffffu, ok)) break;
         }
-        expand_tile(rv, ev, ref_v, gbase + slot_off(2 * g + 1), w, lane);
+        expand_tile(rv, ev_now, ref_v, base + slot_off(2 * g + 1), w, lane);
         if (more) {
-          load_bytes(rv, vb, p.v.stride_tok, (j0 + g + 1) * kBN, key_hi, w, lane);
+          load_bytes(rv, vb, p.v.stride_tok, tok + (g + 1) * kBN, key_hi);
           expand_k(g + 1, 2 * g + 2);
         }
         arrive(kBarPairFull + g % kPairBars);
       }
-    } else if (warp == 1 && lane == 0 && n_kv > 0) {
+    } else if (!kQ8 && warp == 1 && lane == 0 && n_kv > 0) {
       // ---------------------------------------------------------------- TMA producer
       auto load_tile = [&](const CUtensorMap* tm, int it, int kv_tile, uint32_t full_bar) {
         tma_load_4d(base + slot_off(it), tm, full_bar, 0, h, (j0 + kv_tile) * kBN, bk);
@@ -412,51 +455,32 @@ attn_x_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
     }
   } else {
     // ------------------------------------------------------------------ softmax + epilogue
-    const int stage = (warp - 4) >> 2;
+    regs_inc<Roles<kQ8>::kRegsSoftmax>();
+    const int stage = (warp - kSoftmaxWarp0) >> 2;
     if (stage == 0 || two_tiles) {
       const int quad = warp & 3;
       const int row = quad * 32 + lane;
       const uint32_t lane_base = static_cast<uint32_t>(quad * 32) << 16;
       const uint32_t tS = tmem + lane_base + kColS + stage * 128;
       const uint32_t tO = tmem + lane_base + kColO + stage * 128;
-      const int full_lo = kQ8 ? 0 : words[kWordFullLo], full_hi = kQ8 ? key_hi : words[kWordFullHi];
+      const int full_lo = kSpans ? words[kWordFullLo] : 0, full_hi = kSpans ? words[kWordFullHi] : key_hi;
       float m_used = -INFINITY;  // running maximum (lags by up to the threshold); -inf: no key so far
       float l = 0.f;
       int ref_v = 0;  // V exponent the accumulator is in (kQ8)
       bool ok = true;
       for (int j = 0; j < n_kv; ++j) {
-        ok = mbar_wait(bar(kBarSFull + stage), j & 1, abort_flag, p.status, WAIT_S_FULL);
-        if (kQ8 && ok)  // K_j's and V_j's exponents were published with K_j: already complete, read for its ordering
-          ok = j == 0 ? mbar_wait(bar(kBarK0Full), 0, abort_flag, p.status, WAIT_KV_FULL)
-                      : mbar_wait(bar(kBarPairFull + (j - 1) % kPairBars), ((j - 1) / kPairBars) & 1, abort_flag, p.status,
-                                  WAIT_KV_FULL);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        tc_fence_after();
-        uint32_t s[4][32];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld32(tS + c * 32, s[c]);
-        tmem_wait_ld();
         const int key0 = (j0 + j) * kBN;
-        const int lo = kQ8 ? 0 : span_lo - key0, hi = (kQ8 ? key_hi : span_hi) - key0;
-        if (lo > 0 || hi < kBN) {
-          const uint32_t width = static_cast<uint32_t>(max(hi - lo, 0));
-#pragma unroll
-          for (int c = 0; c < 4; ++c)
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (static_cast<uint32_t>(c * 32 + i - lo) >= width) s[c][i] = 0xFF800000u;  // -inf
-        }
         // V rows that no query row of this CTA attends lie inside the tensor, so the TMA did not zero-fill them and they
         // may hold anything, NaN included; P is 0 there, but 0 x NaN would poison output rows.  Query tile 0 clears
-        // them in shared memory before it reports P (tile 1's P V is issued later).  (kQ8: expanded as zeros.)
+        // them in shared memory before it reports P (tile 1's P V is issued later), and before it holds a tile of S in
+        // registers.  (kQ8: expanded as zeros.)
         if (!kQ8 && stage == 0 && (key0 < full_lo || key0 + kBN > full_hi)) {
           ok = mbar_wait(bar(kBarPairFull + j % kPairBars), (j / kPairBars) & 1, abort_flag, p.status, WAIT_KV_FULL);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           const int key = key0 + row;
           const bool in_hull = key >= key_lo && key < key_hi;
-          bool attended = false;
+          bool attended = !kSpans;  // one length per row: every row attends the whole hull
           // rows in a scattered order, so that a few of them usually settle it
           for (int i = 0; i < 2 * kBM && __any_sync(0xffffffffu, in_hull && !attended); ++i) {
             const int r = q0 + ((i * 97) & (2 * kBM - 1));
@@ -474,6 +498,27 @@ attn_x_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
             }
           }
           fence_proxy_async_smem();
+        }
+        ok = mbar_wait(bar(kBarSFull + stage), j & 1, abort_flag, p.status, WAIT_S_FULL);
+        if (kQ8 && ok)  // K_j's and V_j's exponents were published with K_j: already complete, read for its ordering
+          ok = j == 0 ? mbar_wait(bar(kBarK0Full), 0, abort_flag, p.status, WAIT_KV_FULL)
+                      : mbar_wait(bar(kBarPairFull + (j - 1) % kPairBars), ((j - 1) / kPairBars) & 1, abort_flag, p.status,
+                                  WAIT_KV_FULL);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+        uint32_t s[4][32];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld32(tS + c * 32, s[c]);
+        tmem_wait_ld();
+        const int lo = kSpans ? span_lo - key0 : 0, hi = (kSpans ? span_hi : key_hi) - key0;
+        if (__any_sync(0xffffffffu, lo > 0 || hi < kBN)) {
+          const uint32_t width = static_cast<uint32_t>(max(hi - lo, 0));
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (static_cast<uint32_t>(c * 32 + i - lo) >= width) s[c][i] = 0xFF800000u;  // -inf
         }
         float mx0 = -INFINITY, mx1 = -INFINITY, mx2 = -INFINITY, mx3 = -INFINITY;
 #pragma unroll
@@ -613,21 +658,22 @@ attn_x_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
 // Merge the parts of the split tiles.  Block = (split tile, query tile, group of 32 rows); 256 threads = 32 rows x 8
 // column groups of 16.  out = sum_k w_k O_k / sum_k 2^(m_k - m) l_k with w_k = 2^(m_k - m + R_k - R) and the result in
 // units of 2^(R+6); a part without a key has l_k = 0 and no accumulator.
-template <bool kQ8>
+template <int kMode>
 __global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ AttnXParams p) {
+  constexpr bool kQ8 = kMode == kModeExpand, kSpans = kMode == kModeSpans;
   const int stage = blockIdx.y;
   const int row = blockIdx.z * 32 + (threadIdx.x >> 3);
   const int c0 = (threadIdx.x & 7) * 16;
   int first;
-  if (kQ8) {  // the first item of the blockIdx.x-th tail tile
+  if (!kSpans) {  // the first item of the blockIdx.x-th tail tile
     const int tile = p.n_full + blockIdx.x;
     int r = p.rows - 1;
     while (r > 0 && p.tail_tile0[r] > tile) --r;
     first = p.n_full + p.item0[r] + (tile - p.tail_tile0[r]) * p.parts[r];
   } else {
-    first = blockIdx.x * p.split;
+    first = p.n_full + blockIdx.x * p.split;
   }
-  const Item item = find_item<kQ8>(p, first);
+  const Item item = find_item<kSpans>(p, first);
   const int q_row = item.q0 + stage * kBM + row;
   if (item.part < 0 || q_row >= p.q_tokens) return;
   const float* pm = p.part_meta + (static_cast<size_t>(item.slot) * 2 + stage) * (3 * kBM) + row;
@@ -669,39 +715,45 @@ __global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ At
                    pack_bf16x2(acc[8 * i + 4], acc[8 * i + 5]), pack_bf16x2(acc[8 * i + 6], acc[8 * i + 7]));
 }
 
-template <bool kQ8>
+template <int kMode>
 cudaError_t launch(const CUtensorMap& tm_q, const CUtensorMap& tm_k, const CUtensorMap& tm_v, const AttnXParams& p,
                    cudaStream_t stream) {
+  constexpr bool kSpans = kMode == kModeSpans;
   static DynamicSmemGrant smem_grant;  // one per instantiation
   DeviceInfo di;
   cudaError_t e = device_info(&di);
-  if (e == cudaSuccess) e = smem_grant.ensure(attn_x_kernel<kQ8>, static_cast<int>(kSmemBytes), di.device);
+  if (e == cudaSuccess) e = smem_grant.ensure(attn_x_kernel<kMode>, static_cast<int>(kSmemBytes), di.device);
   if (e != cudaSuccess) return e;
-  const int items = kQ8 ? p.n_full + p.n_parts : p.n_tiles * p.split;
-  attn_x_kernel<kQ8><<<items, kThreads, kSmemBytes, stream>>>(tm_q, tm_k, tm_v, p);
+  const int items = p.n_full + p.n_parts;
+  attn_x_kernel<kMode><<<items, Roles<kMode == kModeExpand>::kThreads, kSmemBytes, stream>>>(tm_q, tm_k, tm_v, p);
   e = cudaGetLastError();
-  const int merged = kQ8 ? (p.split > 1 ? p.n_tiles - p.n_full : 0) : (p.split > 1 ? p.n_tiles : 0);
-  if (e != cudaSuccess || merged == 0) return e;
-  combine_kernel<kQ8><<<dim3(merged, p.q_tokens > kBM ? 2 : 1, kBM / 32), 256, 0, stream>>>(p);
+  if (e != cudaSuccess || p.split == 1) return e;
+  const int merged = p.n_tiles - p.n_full;
+  combine_kernel<kMode><<<dim3(merged, p.q_tokens > kBM ? 2 : 1, kBM / 32), 256, 0, stream>>>(p);
   return cudaGetLastError();
 }
 
 }  // namespace attnx
 
-cudaError_t launch_attn_q8(const CUtensorMap& tm_q, const AttnXParams& p, cudaStream_t stream) {
-  return attnx::launch<true>(tm_q, tm_q, tm_q, p, stream);
+cudaError_t launch_attn_q8_expand(const CUtensorMap& tm_q, const AttnXParams& p, cudaStream_t stream) {
+  return attnx::launch<attnx::kModeExpand>(tm_q, tm_q, tm_q, p, stream);
+}
+
+cudaError_t launch_attn_lens(const CUtensorMap& tm_q, const CUtensorMap& tm_k, const CUtensorMap& tm_v,
+                             const AttnXParams& p, cudaStream_t stream) {
+  return attnx::launch<attnx::kModeLens>(tm_q, tm_k, tm_v, p, stream);
 }
 
 cudaError_t launch_attn_spans(const CUtensorMap& tm_q, const CUtensorMap& tm_k, const CUtensorMap& tm_v,
                               const AttnXParams& p, cudaStream_t stream) {
-  return attnx::launch<false>(tm_q, tm_k, tm_v, p, stream);
+  return attnx::launch<attnx::kModeSpans>(tm_q, tm_k, tm_v, p, stream);
 }
 
 // Splitting along the keys.  With one CTA per SM, n_tiles = waves * sms + tail leaves only `tail` SMs busy at the end
 // (all of them, when there are few tiles).  The tail's tiles - those of the shortest rows, rows are taken longest first -
 // are cut into parts of about c key tiles, c the smallest for which the parts still fit one wave.  A part costs its
 // set-up and a pass over its accumulator, so c stays at kMinTiles or more.
-int plan_q8(AttnXParams& p, int sms) {
+int plan_lens(AttnXParams& p, int sms) {
   constexpr int kMinTiles = 8;
   const int per_row = p.pair_tiles * p.heads;
   int n_kv[SDV2_MAX_ROWS], first[SDV2_MAX_ROWS];
@@ -749,16 +801,18 @@ int plan_q8(AttnXParams& p, int sms) {
   return p.split > 1 ? p.n_parts : 0;
 }
 
-// Spans live on the device, so the host splits by the number of tiles and keys alone: parts whose share is empty cost
-// little.
+// Spans live on the device, so the host cuts the tail's tiles by their number and the number of keys alone; a part whose
+// share is empty costs little.  Tiles before the tail run late queries first.
 int plan_spans(AttnXParams& p, int sms) {
   constexpr int kMinTiles = 4;
   const int64_t n_tiles = static_cast<int64_t>(p.pair_tiles) * p.heads * p.rows;
   if (n_tiles > 0x7FFFFFFFLL / 64) return -1;
   p.n_tiles = static_cast<int>(n_tiles);
-  p.split = 1;
-  if (p.n_tiles < sms) p.split = max(1, min(min(sms / p.n_tiles, 64), (p.kv_tokens + 127) / 128 / kMinTiles));
-  return p.split > 1 ? p.n_tiles * p.split : 0;
+  const int tail = p.n_tiles % sms;
+  p.n_full = p.n_tiles - tail;
+  p.split = tail == 0 ? 1 : max(1, min(min(sms / tail, 64), (p.kv_tokens + 127) / 128 / kMinTiles));
+  p.n_parts = tail * p.split;
+  return p.split > 1 ? p.n_parts : 0;
 }
 
 }  // namespace sdv2

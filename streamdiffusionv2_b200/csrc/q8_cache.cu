@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(256) rope_kv_append_q8_kernel(const __grid_con
 __global__ void __launch_bounds__(256) kv_read_q8_kernel(const __grid_constant__ Q8ReadParams p) {
   const int b = blockIdx.y;
   const int t0 = blockIdx.x * p.block_tokens;
-  const int n = min(p.block_tokens, p.tokens - t0) * p.row_vecs;
+  const int n = min(p.block_tokens, p.count[b] - t0) * p.row_vecs;
   for (int i = threadIdx.x; i < n; i += 256) {
     const int j = fast_div(i, p.magic_row_vecs);
     const int r = i - j * p.row_vecs;

@@ -167,6 +167,7 @@ struct Q8ReadParams {
   int row_vecs, block_tokens;  // filled in by the launcher
   uint32_t magic_row_vecs;
   int64_t begin[SDV2_MAX_ROWS];
+  int count[SDV2_MAX_ROWS];  // tokens to read of each row, at most `tokens`
 };
 cudaError_t launch_kv_read_q8(const Q8ReadParams& p, cudaStream_t stream);
 
@@ -181,10 +182,10 @@ struct AttnXParams {
   float* part_o;         // [parts][2][128][128] fp32
   float* part_meta;      // [parts][2][3][128] fp32: running maximum (log2 units), sum, V exponent
   int pair_tiles, n_tiles;
-  int split;             // spans: parts of every tile; 8-bit cache: the most parts of a tile
-  // 8-bit cache: rows longest first; tiles [0, n_full) whole, the others in parts[r] parts, n_parts items in all
+  int n_full, n_parts;   // tiles [0, n_full) run whole, the others in parts, n_parts of them in all
+  int split;             // spans: parts of each of the others; lengths: the most parts of one of them
+  // 8-bit cache, lengths: rows longest first, parts[r] parts for the tiles of a row
   sdv2_view k, v, k_exp, v_exp;
-  int n_full, n_parts;
   int seq_lens[SDV2_MAX_ROWS];     // by row
   int order[SDV2_MAX_ROWS];        // rows, longest first; the arrays below go by place in this order
   int tail_tile0[SDV2_MAX_ROWS], item0[SDV2_MAX_ROWS], parts[SDV2_MAX_ROWS];
@@ -195,9 +196,11 @@ struct AttnXParams {
 };
 constexpr size_t kAttnXPartFloats = 2 * (128 * 128 + 3 * 128);
 // Fill in how the work is cut up; returns the partial-result slots needed (0: none) or -1 (too many tiles).
-int plan_q8(AttnXParams& p, int sms);
+int plan_lens(AttnXParams& p, int sms);
 int plan_spans(AttnXParams& p, int sms);
-cudaError_t launch_attn_q8(const CUtensorMap& tm_q, const AttnXParams& p, cudaStream_t stream);
+cudaError_t launch_attn_q8_expand(const CUtensorMap& tm_q, const AttnXParams& p, cudaStream_t stream);
+cudaError_t launch_attn_lens(const CUtensorMap& tm_q, const CUtensorMap& tm_k, const CUtensorMap& tm_v,
+                             const AttnXParams& p, cudaStream_t stream);
 cudaError_t launch_attn_spans(const CUtensorMap& tm_q, const CUtensorMap& tm_k, const CUtensorMap& tm_v,
                               const AttnXParams& p, cudaStream_t stream);
 

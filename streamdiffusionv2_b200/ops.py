@@ -5,9 +5,9 @@ not synchronise.  There is no CPU or PyTorch fallback: a missing library or a fa
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
 import math
+import struct
 from typing import Dict, Optional, Sequence, Tuple
 
 import torch
@@ -301,35 +301,93 @@ def attn_kvcache_simt(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
     return out
 
 
-def _on_device(t: torch.Tensor):
-    """Context in which a launch goes to `t`'s device, whatever the current one is."""
-    idx = t.device.index
-    return contextlib.nullcontext() if idx == torch.cuda.current_device() else torch.cuda.device(idx)
+def _wrong(what: str, name: str, t: torch.Tensor, shape, dtype, device):
+    return ValueError(f"{what}: {name} must be a {dtype} tensor {list(shape)} on {device} with contiguous head_dim, not "
+                      f"{t.dtype} {list(t.shape)} (strides {list(t.stride())}) on {t.device}")
 
 
-def _check_same(what: str, ref: torch.Tensor, tensors: dict) -> None:
-    for name, (t, shape, dtype) in tensors.items():
-        if tuple(t.shape) != tuple(shape) or t.dtype != dtype or t.device != ref.device:
-            raise ValueError(f"{what}: {name} must be a {dtype} tensor {list(shape)} on {ref.device}, "
-                             f"not {t.dtype} {list(t.shape)} on {t.device}")
+def _view4(what: str, name: str, t: torch.Tensor, shape, dtype, device):
+    """(pointer, row, token and head stride) of a [rows, tokens, heads, head_dim] tensor of exactly this shape, type and
+    device.  A size-1 row dimension may carry any stride: it gets a legal one."""
+    st = t.stride()
+    if t.shape != shape or t.dtype is not dtype or t.device != device or st[3] != 1:
+        raise _wrong(what, name, t, shape, dtype, device)
+    return t.data_ptr(), st[0] if shape[0] > 1 else shape[1] * st[1], st[1], st[2]
 
 
-def _exp_view(t: torch.Tensor) -> N.View:
-    """[rows, tokens, heads] int8 exponents of an 8-bit cache (a size-1 dimension may carry any stride: give it a legal
-    one)."""
-    tok, head = t.stride(1) if t.shape[1] > 1 else max(1, t.shape[2]), t.stride(2) if t.shape[2] > 1 else 1
-    return N.View(t.data_ptr(), t.stride(0) if t.shape[0] > 1 else t.shape[1] * tok, tok, head)
+def _view3(what: str, name: str, t: torch.Tensor, shape, device):
+    """The same for the int8 exponents [rows, tokens, heads] of an 8-bit cache."""
+    if t.shape != shape or t.dtype is not torch.int8 or t.device != device:
+        raise _wrong(what, name, t, shape, torch.int8, device)
+    st = t.stride()
+    tok, head = st[1] if shape[1] > 1 else max(1, shape[2]), st[2] if shape[2] > 1 else 1
+    return t.data_ptr(), st[0] if shape[0] > 1 else shape[1] * tok, tok, head
 
 
-def _check_q8(what: str, ref: torch.Tensor, k_cache, v_cache, k_exp, v_exp, rows: int, heads: int, head_dim: int) -> int:
-    """Shapes, types and devices of an 8-bit cache's four tensors; returns its length in tokens."""
+def _q8_views(what: str, device, k_cache, v_cache, k_exp, v_exp, rows: int, heads: int, head_dim: int):
+    """Length in tokens and the four views of an 8-bit cache."""
     if head_dim != 128:
         raise ValueError(f"{what}: the 8-bit cache has head_dim 128, not {head_dim}")
     smax = k_cache.shape[1] if k_cache.dim() == 4 else 0
-    shape = (rows, smax, heads, head_dim)
-    _check_same(what, ref, {"k_cache": (k_cache, shape, torch.uint8), "v_cache": (v_cache, shape, torch.uint8),
-                            "k_exp": (k_exp, shape[:3], torch.int8), "v_exp": (v_exp, shape[:3], torch.int8)})
-    return smax
+    s4 = (rows, smax, heads, 128)
+    s3 = s4[:3]
+    u8 = torch.uint8
+    return smax, (*_view4(what, "k_cache", k_cache, s4, u8, device), *_view4(what, "v_cache", v_cache, s4, u8, device),
+                  *_view3(what, "k_exp", k_exp, s3, device), *_view3(what, "v_exp", v_exp, s3, device))
+
+
+_VIEWS = {n: (struct.Struct(f"{4 * n}q").pack, C.c_char * (32 * n)) for n in (4, 6, 8)}
+
+
+def _packed_views(*flat):
+    """Views (four numbers each) back to back in memory: the buffer to keep until the launch and their addresses."""
+    pack, buf = _VIEWS[len(flat) >> 2]
+    arr = buf.from_buffer_copy(pack(*flat))
+    base = C.addressof(arr)
+    return arr, range(base, base + 8 * len(flat), 32)
+
+
+def _launch(name: str, work, device: torch.device, fn, args) -> None:
+    """fn(*args, stream) with `device` current, logged under `name` with `work()` units of work."""
+    idx = device.index
+    if idx is None:
+        raise ValueError(f"{name}: expected CUDA tensors (there is no CPU path)")
+    if idx != torch.cuda.current_device():
+        with torch.cuda.device(idx):
+            return _launch(name, work, device, fn, args)
+    stream = torch._C._cuda_getCurrentRawStream(idx)
+    if _log is None:
+        rc = fn(*args, stream)
+    else:
+        with _Logged(name, work()):
+            rc = fn(*args, stream)
+    if rc != 0:
+        N.check(rc, name)
+
+
+def _call_scratch(nbytes_fn, device: torch.device, *args):
+    """(tensor to keep until the launch, pointer, bytes) of a call's own scratch.  It comes from PyTorch's allocator on
+    the launching stream (a graph's own pool while capturing), so calls on other streams and other recorded graphs never
+    share it."""
+    if device.index is not None and device.index != torch.cuda.current_device():
+        with torch.cuda.device(device.index):
+            return _call_scratch(nbytes_fn, device, *args)
+    nbytes = nbytes_fn(*args)
+    if nbytes == 0:
+        return None, None, 0
+    t = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    return t, t.data_ptr(), nbytes
+
+
+def _status_ptr(device: torch.device):
+    """Address of the device's status word (the first word of `workspace`)."""
+    return workspace(device).data_ptr() if device.index is not None else None
+
+
+def _cuda_device(what: str, t: torch.Tensor) -> torch.device:
+    if t.dim() != 4:
+        raise ValueError(f"{what}: expected a [rows, tokens, heads, head_dim] tensor, not {list(t.shape)}")
+    return t.device
 
 
 def q8_cache(rows: int, tokens: int, heads: int, device) -> Dict[str, torch.Tensor]:
@@ -353,27 +411,26 @@ def rope_kv_append_q8(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache
     magnitudes min(rint(|x| / 2^e), 127).  A head vector with a value that is not finite reads back as NaN.
     q, k, v [B, N, H, 128] bf16 or fp32; `index_tensors`, `index_values`, `step_params` as for `rope_kv_append`.
     Returns the roped q, the same bits as `rope_kv_append`'s."""
-    B, n_new, H, D = q.shape
-    smax = _check_q8("rope_kv_append_q8", q, k_cache, v_cache, k_exp, v_exp, B, H, D)
+    what = "rope_kv_append_q8"
+    dev = _cuda_device(what, q)
+    shape, dtype = q.shape, q.dtype
+    B, n_new, H, D = shape
+    smax, cache = _q8_views(what, dev, k_cache, v_cache, k_exp, v_exp, B, H, D)
     if q_out is None:
-        q_out = torch.empty((B, n_new, H, D), dtype=q.dtype, device=q.device)
-    _check_same("rope_kv_append_q8", q, {"k": (k, q.shape, q.dtype), "v": (v, q.shape, q.dtype),
-                                         "q_out": (q_out, q.shape, q.dtype),
-                                         "table": (table, (table.shape[0], D // 2, 2), torch.float64)})
-    if not table.is_contiguous():
-        raise ValueError("rope_kv_append_q8: the rope table must be contiguous")
-    f, h, w = (int(x) for x in grid)
-    ge_dev = le_dev = ge_val = le_val = params = None
+        q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    if (table.dim() != 3 or table.shape[1:] != (D // 2, 2) or table.dtype is not torch.float64 or table.device != dev
+            or not table.is_contiguous()):
+        raise ValueError(f"{what}: the rope table must be a contiguous float64 [rows, {D // 2}, 2] tensor on {dev}")
+    f, h, w = grid
+    ge_dev = le_dev = ge_val = le_val = params = starts = dsts = None
     if index_tensors is not None:
-        g, l = index_tensors
-        for t in (g, l):
-            if t.dtype != torch.int64 or t.numel() < B or not t.is_contiguous() or t.device != q.device:
+        for t in index_tensors:
+            if t.dtype is not torch.int64 or t.numel() < B or not t.is_contiguous() or t.device != dev:
                 raise ValueError("index tensors must be contiguous int64 with one entry per row, on q's device")
-        ge_dev, le_dev = g.data_ptr(), l.data_ptr()
-    starts = dsts = None
+        ge_dev, le_dev = index_tensors[0].data_ptr(), index_tensors[1].data_ptr()
     if step_params is not None:
-        if (step_params.dtype != torch.int64 or not step_params.is_contiguous() or step_params.numel() != 4 * B
-                or step_params.device != q.device):
+        if (step_params.dtype is not torch.int64 or not step_params.is_contiguous() or step_params.numel() != 4 * B
+                or step_params.device != dev):
             raise ValueError("step_params must be a contiguous int64 [4, rows] tensor on the same device")
         params = step_params.data_ptr()
     else:
@@ -384,14 +441,12 @@ def rope_kv_append_q8(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache
             if index_values is None or len(index_values[0]) < B or len(index_values[1]) < B:
                 raise ValueError("index_values need one entry per row")
             ge_val, le_val = N.i64_array(index_values[0]), N.i64_array(index_values[1])
-    views = [N.view(t) for t in (q, k, v, q_out, k_cache, v_cache)] + [_exp_view(k_exp), _exp_view(v_exp)]
-    args = [*[C.byref(x) for x in views], B, n_new, H, D, smax, table.data_ptr(), table.shape[0], f, h, w, starts, dsts,
-            params, ge_dev, le_dev, ge_val, le_val, N.dtype_code(q.dtype), workspace(q.device).data_ptr(),
-            N.stream_ptr(q.device)]
-    fn = N.lib().sdv2_rope_kv_append_q8
-    with _on_device(q), _Logged("rope_kv_append_q8", B * n_new * H * (4.0 * D * q.element_size() + 2 * (D + 1))):
-        rc = fn(*args)
-    N.check(rc, "sdv2_rope_kv_append_q8")
+    keep, at = _packed_views(*_view4(what, "q", q, shape, dtype, dev), *_view4(what, "k", k, shape, dtype, dev),
+                             *_view4(what, "v", v, shape, dtype, dev), *_view4(what, "q_out", q_out, shape, dtype, dev),
+                             *cache)
+    _launch(what, lambda: B * n_new * H * (4.0 * D * q.element_size() + 2 * (D + 1)), dev, N.lib().sdv2_rope_kv_append_q8,
+            (*at, B, n_new, H, D, smax, table.data_ptr(), table.shape[0], int(f), int(h), int(w), starts, dsts, params, ge_dev,
+             le_dev, ge_val, le_val, N.dtype_code(dtype), _status_ptr(dev)))
     return q_out
 
 
@@ -400,20 +455,20 @@ def kv_read_q8(k_cache: torch.Tensor, v_cache: torch.Tensor, k_exp: torch.Tensor
                out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """(k, v) [B, tokens, H, 128]: what an 8-bit cache holds of tokens begin[b] .. begin[b] + tokens - 1 of every row,
     in bf16 or fp32 (both exact)."""
+    what = "kv_read_q8"
+    dev = _cuda_device(what, k_cache)
     B, _, H, D = k_cache.shape
-    smax = _check_q8("kv_read_q8", k_cache, k_cache, v_cache, k_exp, v_exp, B, H, D)
-    if out is None:
-        out = tuple(torch.empty((B, tokens, H, D), dtype=dtype, device=k_cache.device) for _ in range(2))
-    _check_same("kv_read_q8", k_cache, {"out[0]": (out[0], (B, tokens, H, D), dtype), "out[1]": (out[1], (B, tokens, H, D), dtype)})
+    smax, cache = _q8_views(what, dev, k_cache, v_cache, k_exp, v_exp, B, H, D)
+    shape = (B, tokens, H, D)
     if len(begin) < B:
         raise ValueError("kv_read_q8: begin needs one entry per row")
-    if out[0].numel() == 0:
-        return out
-    views = [N.view(t) for t in (k_cache, v_cache)] + [_exp_view(k_exp), _exp_view(v_exp)] + [N.view(t) for t in out]
-    with _on_device(k_cache), _Logged("kv_read_q8", B * tokens * H * 2.0 * (D + 1 + D * out[0].element_size())):
-        rc = N.lib().sdv2_kv_read_q8(*[C.byref(x) for x in views], B, tokens, H, D, smax, N.i64_array(begin),
-                                     N.dtype_code(dtype), N.stream_ptr(k_cache.device))
-    N.check(rc, "sdv2_kv_read_q8")
+    if out is None:
+        out = torch.empty((2,) + shape, dtype=dtype, device=dev).unbind(0)
+    keep, at = _packed_views(*cache, *_view4(what, "out[0]", out[0], shape, dtype, dev),
+                             *_view4(what, "out[1]", out[1], shape, dtype, dev))
+    if B * tokens * H != 0:
+        _launch(what, lambda: B * tokens * H * 2.0 * (D + 1 + D * out[0].element_size()), dev, N.lib().sdv2_kv_read_q8,
+                (*at, B, tokens, H, D, smax, N.i64_array(begin), N.dtype_code(dtype)))
     return out
 
 
@@ -422,39 +477,27 @@ def attn_kvcache_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
                     softmax_scale: Optional[float] = None) -> torch.Tensor:
     """`attn_kvcache` over an 8-bit cache: softmax(q k^T scale) v over the values that cache[b, :seq_lens[b]] holds
     (bf16 q and output).  seq_lens[b] may be 0: that row's output is 0."""
-    B, n_q, H, D = q.shape
-    if q.dtype != torch.bfloat16:
+    what = "attn_kvcache_q8"
+    dev = _cuda_device(what, q)
+    shape = q.shape
+    B, n_q, H, D = shape
+    if q.dtype is not torch.bfloat16:
         raise ValueError("the tensor-core attention kernel takes bf16")
-    smax = _check_q8("attn_kvcache_q8", q, k_cache, v_cache, k_exp, v_exp, B, H, D)
+    smax, cache = _q8_views(what, dev, k_cache, v_cache, k_exp, v_exp, B, H, D)
     if out is None:
-        out = torch.empty((B, n_q, H, D), dtype=q.dtype, device=q.device)
-    _check_same("attn_kvcache_q8", q, {"out": (out, q.shape, q.dtype)})
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     if len(seq_lens) < B:
         raise ValueError("attn_kvcache_q8: seq_lens needs one entry per row")
+    keep, at = _packed_views(*_view4(what, "q", q, shape, q.dtype, dev), *cache, *_view4(what, "out", out, shape, q.dtype, dev))
     if q.numel() == 0 or smax == 0:
         return out.zero_()
     scale = softmax_scale if softmax_scale is not None else 1.0 / math.sqrt(D)
     lens = N.i32_array(seq_lens)
-    views = [N.view(t) for t in (q, k_cache, v_cache)] + [_exp_view(k_exp), _exp_view(v_exp), N.view(out)]
-    with _on_device(q):
-        lib = N.lib()
-        scratch = _scratch(lib.sdv2_attn_q8_scratch_bytes(B, n_q, H, smax, lens), q.device)
-        args = [*[C.byref(x) for x in views], B, n_q, H, D, smax, lens, scale, *scratch[1:], workspace(q.device).data_ptr(),
-                N.stream_ptr(q.device)]
-        with _Logged("attn_kvcache_q8", 4.0 * n_q * D * H * float(sum(int(x) for x in seq_lens[:B]))):
-            rc = lib.sdv2_attn_kvcache_q8(*args)
-    N.check(rc, "sdv2_attn_kvcache_q8")
+    lib = N.lib()
+    scratch = _call_scratch(lib.sdv2_attn_q8_scratch_bytes, dev, B, n_q, H, smax, lens)
+    _launch(what, lambda: 4.0 * n_q * D * H * float(sum(int(x) for x in seq_lens[:B])), dev, lib.sdv2_attn_kvcache_q8,
+            (*at, B, n_q, H, D, smax, lens, scale, scratch[1], scratch[2], _status_ptr(dev)))
     return out
-
-
-def _scratch(nbytes: int, device):
-    """(tensor to keep until the launch, pointer, bytes) of a call's own scratch.  It comes from PyTorch's allocator on
-    the launching stream (a graph's own pool while capturing), so calls on other streams and other recorded graphs never
-    share it."""
-    if nbytes == 0:
-        return None, None, 0
-    t = torch.empty(nbytes, dtype=torch.uint8, device=device)
-    return t, t.data_ptr(), nbytes
 
 
 def attn_spans(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, begin: Optional[torch.Tensor], end: torch.Tensor, *,
@@ -464,30 +507,30 @@ def attn_spans(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, begin: Optiona
     stride-0 expands over rows); begin (None: 0) and end int32 [B, N] on the device, any strides (an expanded [B, 1]
     does for one span per row).  Spans are clipped to the keys there are; a query with an empty span gets 0.  K and V of
     keys that no query attends may hold anything."""
-    B, n_q, H, D = q.shape
-    if q.dtype != torch.bfloat16:
+    what = "attn_spans"
+    dev = _cuda_device(what, q)
+    shape, dtype = q.shape, q.dtype
+    B, n_q, H, D = shape
+    if dtype is not torch.bfloat16:
         raise ValueError("the tensor-core attention kernel takes bf16")
     S = k.shape[1]
+    kv_shape = (B, S, H, D)
     if out is None:
-        out = torch.empty((B, n_q, H, D), dtype=q.dtype, device=q.device)
-    wanted = {"k": (k, (B, S, H, D), q.dtype), "v": (v, (B, S, H, D), q.dtype), "out": (out, q.shape, q.dtype),
-              "end": (end, (B, n_q), torch.int32)}
-    if begin is not None:
-        wanted["begin"] = (begin, (B, n_q), torch.int32)
-    _check_same("attn_spans", q, wanted)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    for name, t in (("end", end), ("begin", begin)):
+        if t is not None and (t.shape != (B, n_q) or t.dtype is not torch.int32 or t.device != dev):
+            raise ValueError(f"attn_spans: {name} must be an int32 tensor {[B, n_q]} on {dev}")
+    keep, at = _packed_views(*_view4(what, "q", q, shape, dtype, dev), *_view4(what, "k", k, kv_shape, dtype, dev),
+                             *_view4(what, "v", v, kv_shape, dtype, dev), *_view4(what, "out", out, shape, dtype, dev))
     if q.numel() == 0 or S == 0:
         return out.zero_()
     scale = softmax_scale if softmax_scale is not None else 1.0 / math.sqrt(D)
-    views = [N.view(t) for t in (q, k, v, out)]
-    b_args = (None, 0, 0) if begin is None else (begin.data_ptr(), *begin.stride())
-    with _on_device(q):
-        lib = N.lib()
-        scratch = _scratch(lib.sdv2_attn_spans_scratch_bytes(B, n_q, H, S), q.device)
-        args = [*[C.byref(x) for x in views], B, n_q, H, D, S, *b_args, end.data_ptr(), *end.stride(), scale, *scratch[1:],
-                workspace(q.device).data_ptr(), N.stream_ptr(q.device)]
-        with _Logged("attn_spans"):
-            rc = lib.sdv2_attn_spans(*args)
-    N.check(rc, "sdv2_attn_spans")
+    lib = N.lib()
+    scratch = _call_scratch(lib.sdv2_attn_spans_scratch_bytes, dev, B, n_q, H, S)
+    spans = (None, 0, 0) if begin is None else (begin.data_ptr(), *begin.stride())
+    _launch(what, lambda: 4.0 * B * n_q * D * H * S, dev, lib.sdv2_attn_spans,
+            (*at, B, n_q, H, D, S, *spans, end.data_ptr(), *end.stride(), scale, scratch[1], scratch[2],
+             _status_ptr(dev)))
     return out
 
 
