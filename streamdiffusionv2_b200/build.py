@@ -13,8 +13,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libsdv2.so")
 SOURCES = ["api.cu", "rope_append.cu", "attn_simt.cu", "attn_tcgen05.cu", "noalloc.cu", "block_elementwise.cu", "ring_plan.cu", "q8_cache.cu",
-           "attn_q8_spans.cu"]
-HEADERS = ["ptx.cuh", "attn_tiles.cuh", "rope_append.cuh", "q8.cuh", "sdv2_internal.h", os.path.join("..", "..", "include", "sdv2.h")]
+           "attn_q8_spans.cu", "attn_q8_few.cu"]
+HEADERS = ["ptx.cuh", "attn_items.cuh", "attn_tiles.cuh", "rope_append.cuh", "q8.cuh", "sdv2_internal.h", os.path.join("..", "..", "include", "sdv2.h")]
 
 
 def _nvcc() -> str:

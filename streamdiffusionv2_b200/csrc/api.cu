@@ -105,6 +105,26 @@ int make_tile_map(CUtensorMap* tm, const sdv2_view* v, int rows, int64_t tokens,
   return SDV2_OK;
 }
 
+// 8-bit cache [rows, tokens, heads, 128] bytes -> 4-D map, box 128 x 1 x box_tokens x 1, 128-byte swizzle.
+int make_byte_map(CUtensorMap* tm, const sdv2_view* v, int rows, int64_t tokens, int heads, int box_tokens) {
+  auto fn = encode_fn();
+  if (fn == nullptr) return cuda_fail(cudaErrorSymbolNotFound);
+  const int64_t row_stride = v->stride_row > 0 ? v->stride_row : v->stride_tok * tokens;
+  cuuint64_t dims[4] = {128, static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(tokens),
+                        static_cast<cuuint64_t>(v->stride_row > 0 ? rows : 1)};
+  cuuint64_t strides[3] = {static_cast<cuuint64_t>(v->stride_head), static_cast<cuuint64_t>(v->stride_tok),
+                           static_cast<cuuint64_t>(row_stride)};
+  cuuint32_t box[4] = {128, 1, static_cast<cuuint32_t>(box_tokens), 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  CUresult r = fn(tm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, v->ptr, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    g_last_cuda_error = static_cast<int>(r);
+    return SDV2_ERR_CUDA;
+  }
+  return SDV2_OK;
+}
+
 int make_square_map(CUtensorMap* tm, const void* ptr) {
   auto fn = encode_fn();
   if (fn == nullptr) return cuda_fail(cudaErrorSymbolNotFound);
@@ -566,6 +586,8 @@ static int fill_q_out(sdv2::AttnXParams& p, const sdv2_view* q, const sdv2_view*
   return SDV2_OK;
 }
 
+static size_t few_bytes(int slots) { return slots * static_cast<size_t>(sdv2::kFewRows) * (128 + 2) * sizeof(float); }
+
 static size_t partial_bytes(int slots) { return slots * sdv2::kAttnXPartFloats * sizeof(float); }
 
 static void set_partials(sdv2::AttnXParams& p, void* scratch, int slots) {
@@ -578,8 +600,12 @@ static void set_partials(sdv2::AttnXParams& p, void* scratch, int slots) {
 // expanding them to bf16 scratch first costs 6 bytes of HBM traffic a value once, 3900 cycles' share of a key tile.  So
 // from four pairs of query tiles on (more than 768 queries) the cache is expanded first, a group of heads at a time so
 // that the scratch stays near 1 GiB.
+//
+// Up to kFewQueries queries have a kernel of their own that never leaves the cache's bytes for shared-memory tiles.
+constexpr int kFewQueries = 32;
 struct Q8Run {
   sdv2::AttnXParams p;  // of one head group when expanding first
+  bool few;
   int group, longest;
   int slots;        // partial-result slots of the group size that needs the most
   size_t expanded;  // bytes of K, and of V, for one head group
@@ -591,11 +617,13 @@ static int fill_q8(Q8Run& r, int rows, int q_tokens, int heads, int64_t cache_to
   int rc;
   if ((rc = fill_attn_x(r.p, rows, q_tokens, heads, cache_tokens)) != SDV2_OK || (rc = fill_lens(r.p, seq_lens)) != SDV2_OK)
     return rc;
+  r.few = q_tokens <= kFewQueries;
+  if (r.few) r.p.pair_tiles = (q_tokens + sdv2::kFewRows - 1) / sdv2::kFewRows;
   r.group = heads;
   r.longest = 0;
   r.expanded = 0;
   for (int b = 0; b < rows; ++b) r.longest = r.longest > seq_lens[b] ? r.longest : seq_lens[b];
-  if (r.p.pair_tiles >= kExpandFirstPairTiles && r.longest > 0) {
+  if (!r.few && r.p.pair_tiles >= kExpandFirstPairTiles && r.longest > 0) {
     const int64_t per_head = static_cast<int64_t>(rows) * r.longest * 256;
     const int64_t fit = kGroupBytes / per_head;
     r.group = fit >= heads ? heads : (fit < 1 ? 1 : static_cast<int>(fit));
@@ -609,13 +637,14 @@ static int plan_q8(Q8Run& r, int heads) {
   sdv2::DeviceInfo di;
   const cudaError_t e = sdv2::device_info(&di);
   if (e != cudaSuccess) return cuda_fail(e);
+  const int wave = r.few ? di.sms * sdv2::kFewBlocksPerSm : di.sms, min_tiles = r.few ? 2 : 8;
   int last = 0;
   if (heads % r.group != 0) {  // a smaller last group
     r.p.heads = heads % r.group;
-    last = sdv2::plan_lens(r.p, di.sms);
+    last = sdv2::plan_lens(r.p, wave, min_tiles);
   }
   r.p.heads = r.group;
-  r.slots = sdv2::plan_lens(r.p, di.sms);
+  r.slots = sdv2::plan_lens(r.p, wave, min_tiles);
   if (r.slots < 0 || last < 0) return SDV2_ERR_UNSUPPORTED_SHAPE;
   if (last > r.slots) r.slots = last;
   return SDV2_OK;
@@ -624,7 +653,7 @@ static int plan_q8(Q8Run& r, int heads) {
 size_t sdv2_attn_q8_scratch_bytes(int rows, int q_tokens, int heads, int64_t cache_tokens, const int32_t* seq_lens) {
   Q8Run r;
   if (fill_q8(r, rows, q_tokens, heads, cache_tokens, seq_lens) != SDV2_OK || plan_q8(r, heads) != SDV2_OK) return 0;
-  return 2 * r.expanded + partial_bytes(r.slots);
+  return 2 * r.expanded + (r.few ? few_bytes(r.slots) : partial_bytes(r.slots));
 }
 
 int sdv2_attn_kvcache_q8(const sdv2_view* q, const sdv2_view* k_cache, const sdv2_view* v_cache, const sdv2_view* k_exp,
@@ -638,7 +667,7 @@ int sdv2_attn_kvcache_q8(const sdv2_view* q, const sdv2_view* k_cache, const sdv
   if ((rc = fill_q8(r, rows, q_tokens, heads, cache_tokens, seq_lens)) != SDV2_OK) return rc;
   if ((rc = fill_q_out(r.p, q, out, head_dim, softmax_scale, status_dev)) != SDV2_OK) return rc;
   if ((rc = plan_q8(r, heads)) != SDV2_OK) return rc;
-  const size_t need = 2 * r.expanded + partial_bytes(r.slots);
+  const size_t need = 2 * r.expanded + (r.few ? few_bytes(r.slots) : partial_bytes(r.slots));
   if (need > 0 && (scratch_dev == nullptr || scratch_bytes < need)) return SDV2_ERR_WORKSPACE;
   if (!aligned16(scratch_dev)) return SDV2_ERR_MISALIGNED;
   char* scratch = static_cast<char*>(scratch_dev);
@@ -646,8 +675,17 @@ int sdv2_attn_kvcache_q8(const sdv2_view* q, const sdv2_view* k_cache, const sdv
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   CUtensorMap tm_q, tm_k, tm_v;
   cudaError_t e = cudaSuccess;
+  r.p.q = *q; r.p.k = *k_cache; r.p.v = *v_cache; r.p.k_exp = *k_exp; r.p.v_exp = *v_exp;
+  if (r.few) {
+    if (r.slots > 0) r.p.part_meta = r.p.part_o + static_cast<size_t>(r.slots) * sdv2::kFewRows * 128;
+    r.p.k_row_mask = k_cache->stride_row > 0 ? -1 : 0;
+    r.p.v_row_mask = v_cache->stride_row > 0 ? -1 : 0;
+    if ((rc = make_byte_map(&tm_k, k_cache, rows, cache_tokens, heads, 16)) != SDV2_OK) return rc;
+    if ((rc = make_byte_map(&tm_v, v_cache, rows, cache_tokens, heads, 16)) != SDV2_OK) return rc;
+    e = sdv2::launch_attn_few(tm_k, tm_v, r.p, s);
+    return e == cudaSuccess ? SDV2_OK : cuda_fail(e);
+  }
   if (r.expanded == 0) {
-    r.p.k = *k_cache; r.p.v = *v_cache; r.p.k_exp = *k_exp; r.p.v_exp = *v_exp;
     if ((rc = make_tile_map(&tm_q, q, rows, q_tokens, heads)) != SDV2_OK) return rc;
     e = sdv2::launch_attn_q8_expand(tm_q, r.p, s);
     return e == cudaSuccess ? SDV2_OK : cuda_fail(e);
@@ -673,7 +711,7 @@ int sdv2_attn_kvcache_q8(const sdv2_view* q, const sdv2_view* k_cache, const sdv
       sdv2::DeviceInfo di;
       if ((e = sdv2::device_info(&di)) != cudaSuccess) return cuda_fail(e);
       r.p.heads = n;
-      if (sdv2::plan_lens(r.p, di.sms) < 0) return SDV2_ERR_UNSUPPORTED_SHAPE;
+      if (sdv2::plan_lens(r.p, di.sms, 8) < 0) return SDV2_ERR_UNSUPPORTED_SHAPE;
     }
     if ((rc = make_tile_map(&tm_q, &qg, rows, q_tokens, n)) != SDV2_OK) return rc;
     if ((rc = make_tile_map(&tm_k, &kx, rows, r.longest, n)) != SDV2_OK) return rc;

@@ -22,6 +22,7 @@
 #include <math.h>
 #include <stdint.h>
 
+#include "attn_items.cuh"
 #include "attn_tiles.cuh"
 #include "ptx.cuh"
 #include "q8.cuh"
@@ -85,10 +86,6 @@ static_assert(kNumBars * 8 + kNumWords * 4 <= 256, "barrier block too small");
 static_assert(kRing >= 5, "pair g overwrites the tiles of pairs g-3 and g-2: needs five slots");
 
 constexpr float kRescaleThreshold = 8.0f;  // log2 units
-
-__device__ __forceinline__ float exp2_int(int e) {  // 2^e, e clamped to fp32's normal range
-  return __int_as_float((min(max(e, -126), 127) + 127) << 23);
-}
 
 // ------------------------------------------------------------------ expanding the 8-bit cache (kQ8)
 // A tile is 8 steps x 4 warps of four tokens.  A lane has 16 bytes of one token: in every eight lanes, 64 bytes of an
@@ -167,49 +164,25 @@ __device__ __forceinline__ void expand_tile(const TileBytes& t, uint32_t exps, i
 }
 
 // ------------------------------------------------------------------ the kernel
-struct Item {
-  int b, h, q0, part, parts, slot;  // part < 0: the whole key range, written to the output directly
-};
-
 template <bool kSpans>
 __device__ __forceinline__ Item find_item(const AttnXParams& p, int i) {
+  if (!kSpans) return find_item_lens(p, i);
+  // late query tiles first: with masks that grow along the sequence they are the long ones
   Item it;
-  int pt, hb;
+  int tile = i;
   it.part = -1;
   it.parts = 1;
   it.slot = 0;
-  if (!kSpans) {
-    int tile = i, r = 0;
-    if (i >= p.n_full) {
-      const int k = i - p.n_full;
-      r = p.rows - 1;
-      while (r > 0 && p.item0[r] > k) --r;
-      it.parts = p.parts[r];
-      const int local = k - p.item0[r];
-      tile = p.tail_tile0[r] + local / it.parts;
-      if (it.parts > 1) it.part = local % it.parts;
-      it.slot = k;
-    }
-    pt = tile % p.pair_tiles;
-    hb = tile / p.pair_tiles;
-    it.h = hb % p.heads;
-    it.b = p.order[hb / p.heads];
-  } else {
-    // late query tiles first: with masks that grow along the sequence they are the long ones
-    int tile = i;
-    if (i >= p.n_full) {
-      it.slot = i - p.n_full;
-      tile = p.n_full + it.slot / p.split;
-      it.parts = p.split;
-      if (p.split > 1) it.part = it.slot % p.split;
-    }
-    const int per = p.heads * p.rows;
-    pt = p.pair_tiles - 1 - tile / per;
-    hb = tile % per;
-    it.h = hb % p.heads;
-    it.b = hb / p.heads;
+  if (i >= p.n_full) {
+    it.slot = i - p.n_full;
+    tile = p.n_full + it.slot / p.split;
+    it.parts = p.split;
+    if (p.split > 1) it.part = it.slot % p.split;
   }
-  it.q0 = pt * (2 * kBM);
+  const int per = p.heads * p.rows;
+  it.tile = p.pair_tiles - 1 - tile / per;
+  it.h = tile % per % p.heads;
+  it.b = tile % per / p.heads;
   return it;
 }
 
@@ -230,7 +203,7 @@ attn_x_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
   const int lane = threadIdx.x & 31;
   const Item item = find_item<kSpans>(p, blockIdx.x);
-  const int b = item.b, h = item.h, q0 = item.q0;
+  const int b = item.b, h = item.h, q0 = item.tile * (2 * kBM);
   const bool two_tiles = q0 + kBM < p.q_tokens;
   const int bk = p.kv_row_broadcast ? 0 : b;
 
@@ -664,17 +637,9 @@ __global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ At
   const int stage = blockIdx.y;
   const int row = blockIdx.z * 32 + (threadIdx.x >> 3);
   const int c0 = (threadIdx.x & 7) * 16;
-  int first;
-  if (!kSpans) {  // the first item of the blockIdx.x-th tail tile
-    const int tile = p.n_full + blockIdx.x;
-    int r = p.rows - 1;
-    while (r > 0 && p.tail_tile0[r] > tile) --r;
-    first = p.n_full + p.item0[r] + (tile - p.tail_tile0[r]) * p.parts[r];
-  } else {
-    first = p.n_full + blockIdx.x * p.split;
-  }
-  const Item item = find_item<kSpans>(p, first);
-  const int q_row = item.q0 + stage * kBM + row;
+  const Item item =
+      find_item<kSpans>(p, kSpans ? p.n_full + static_cast<int>(blockIdx.x) * p.split : first_item_lens(p, blockIdx.x));
+  const int q_row = item.tile * (2 * kBM) + stage * kBM + row;
   if (item.part < 0 || q_row >= p.q_tokens) return;
   const float* pm = p.part_meta + (static_cast<size_t>(item.slot) * 2 + stage) * (3 * kBM) + row;
   const float* po = p.part_o + (static_cast<size_t>(item.slot) * 2 + stage) * (kBM * kHD) + row * kHD + c0;
@@ -747,58 +712,6 @@ cudaError_t launch_attn_lens(const CUtensorMap& tm_q, const CUtensorMap& tm_k, c
 cudaError_t launch_attn_spans(const CUtensorMap& tm_q, const CUtensorMap& tm_k, const CUtensorMap& tm_v,
                               const AttnXParams& p, cudaStream_t stream) {
   return attnx::launch<attnx::kModeSpans>(tm_q, tm_k, tm_v, p, stream);
-}
-
-// Splitting along the keys.  With one CTA per SM, n_tiles = waves * sms + tail leaves only `tail` SMs busy at the end
-// (all of them, when there are few tiles).  The tail's tiles - those of the shortest rows, rows are taken longest first -
-// are cut into parts of about c key tiles, c the smallest for which the parts still fit one wave.  A part costs its
-// set-up and a pass over its accumulator, so c stays at kMinTiles or more.
-int plan_lens(AttnXParams& p, int sms) {
-  constexpr int kMinTiles = 8;
-  const int per_row = p.pair_tiles * p.heads;
-  int n_kv[SDV2_MAX_ROWS], first[SDV2_MAX_ROWS];
-  for (int r = 0; r < p.rows; ++r) {  // insertion sort, longest row first
-    int at = r;
-    while (at > 0 && p.seq_lens[p.order[at - 1]] < p.seq_lens[r]) {
-      p.order[at] = p.order[at - 1];
-      --at;
-    }
-    p.order[at] = r;
-  }
-  const int64_t n_tiles = static_cast<int64_t>(per_row) * p.rows;
-  if (n_tiles > 0x7FFFFFFFLL / 64) return -1;
-  p.n_tiles = static_cast<int>(n_tiles);
-  p.n_full = p.n_tiles - p.n_tiles % sms;
-  int longest = 0;
-  for (int r = 0; r < p.rows; ++r) {
-    n_kv[r] = (p.seq_lens[p.order[r]] + 127) / 128;
-    first[r] = max(r * per_row, p.n_full);
-    if ((r + 1) * per_row > p.n_full) longest = max(longest, n_kv[r]);
-  }
-  auto parts_at = [&](int c, int r) { return n_kv[r] <= c ? 1 : (n_kv[r] + c - 1) / c; };
-  auto items_at = [&](int c) {
-    int64_t n = 0;
-    for (int r = 0; r < p.rows; ++r) n += static_cast<int64_t>(max((r + 1) * per_row - first[r], 0)) * parts_at(c, r);
-    return n;
-  };
-  int lo = kMinTiles, hi = max(longest, kMinTiles);  // the smallest c in [lo, hi] whose parts fit; hi always does
-  while (lo < hi) {
-    const int c = (lo + hi) / 2;
-    if (items_at(c) <= sms) hi = c;
-    else lo = c + 1;
-  }
-  p.split = 1;
-  int item = 0;
-  for (int r = 0; r < p.rows; ++r) {
-    p.tail_tile0[r] = first[r];
-    p.item0[r] = item;
-    p.parts[r] = parts_at(lo, r);
-    const int tiles = max((r + 1) * per_row - first[r], 0);
-    if (tiles > 0) p.split = max(p.split, p.parts[r]);
-    item += tiles * p.parts[r];
-  }
-  p.n_parts = item;
-  return p.split > 1 ? p.n_parts : 0;
 }
 
 // Spans live on the device, so the host cuts the tail's tiles by their number and the number of keys alone; a part whose

@@ -147,6 +147,22 @@ __device__ __forceinline__ uint32_t rms_scale_pair(uint32_t x, float rstd, uint3
 }
 #endif
 
+// Launch `kernel` so that its set-up overlaps the end of the kernel before it on the stream; it has to wait for that
+// kernel's results with griddepcontrol.wait.
+template <typename... Params, typename... Args>
+cudaError_t launch_dependent(void (*kernel)(Params...), dim3 grid, dim3 block, cudaStream_t stream, const Args&... args) {
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = grid;
+  config.blockDim = block;
+  config.stream = stream;
+  config.attrs = &attr;
+  config.numAttrs = 1;
+  return cudaLaunchKernelEx(&config, kernel, args...);
+}
+
 // Records a failing CUDA call for sdv2_last_cuda_error() and returns SDV2_ERR_CUDA.
 int record_cuda_error(cudaError_t e);
 
@@ -185,7 +201,8 @@ struct AttnXParams {
   int n_full, n_parts;   // tiles [0, n_full) run whole, the others in parts, n_parts of them in all
   int split;             // spans: parts of each of the others; lengths: the most parts of one of them
   // 8-bit cache, lengths: rows longest first, parts[r] parts for the tiles of a row
-  sdv2_view k, v, k_exp, v_exp;
+  sdv2_view q, k, v, k_exp, v_exp;
+  int k_row_mask, v_row_mask;      // 0: every row reads row 0 of K / V, else all ones
   int seq_lens[SDV2_MAX_ROWS];     // by row
   int order[SDV2_MAX_ROWS];        // rows, longest first; the arrays below go by place in this order
   int tail_tile0[SDV2_MAX_ROWS], item0[SDV2_MAX_ROWS], parts[SDV2_MAX_ROWS];
@@ -196,8 +213,11 @@ struct AttnXParams {
 };
 constexpr size_t kAttnXPartFloats = 2 * (128 * 128 + 3 * 128);
 // Fill in how the work is cut up; returns the partial-result slots needed (0: none) or -1 (too many tiles).
-int plan_lens(AttnXParams& p, int sms);
+int plan_lens(AttnXParams& p, int wave, int min_tiles);
 int plan_spans(AttnXParams& p, int sms);
+constexpr int kFewRows = 16;        // query rows of a block of launch_attn_few; partials: [parts][16][128], [parts][2][16]
+constexpr int kFewBlocksPerSm = 3;
+cudaError_t launch_attn_few(const CUtensorMap& tm_k, const CUtensorMap& tm_v, const AttnXParams& p, cudaStream_t stream);
 cudaError_t launch_attn_q8_expand(const CUtensorMap& tm_q, const AttnXParams& p, cudaStream_t stream);
 cudaError_t launch_attn_lens(const CUtensorMap& tm_q, const CUtensorMap& tm_k, const CUtensorMap& tm_v,
                              const AttnXParams& p, cudaStream_t stream);

@@ -199,6 +199,7 @@ def _check_q8(c, q, lens, out, scale=None):
 
 @pytest.mark.parametrize("queries,heads,cache,lens", [
     (1, 1, 1, [1]), (1, 2, 130, [130, 0]), (1, 12, 5000, [5000, 4999, 1, 0]), (2, 3, 300, [129]), (16, 2, 2000, [1999, 1]),
+    (17, 2, 300, [299, 16]), (32, 3, 3111, [3111, 64, 15]), (33, 1, 200, [200]), (5, 70, 400, [400, 399, 17, 0, 128]),
     (48, 2, 700, [127, 128, 129]), (100, 2, 300, [300]), (128, 1, 128, [128]), (129, 1, 256, [255]), (256, 2, 1000, [1000, 517]),
     (257, 1, 640, [640]), (300, 3, 1100, [1000, 0, 1100, 3]), (1479, 5, 2100, [2047, 2048]), (3120, 2, 4680, [4680]),
     (700, 40, 600, [600, 385]),                            # more tiles than multiprocessors: whole tiles and a split tail
@@ -252,6 +253,28 @@ def test_q8_attention_exponents_far_apart(queries):
     assert bool(torch.isnan(out[:, :, 2]).all())
     sub = {n: t[:, :, :2] for n, t in c.items()}
     _check_q8(sub, q[:, :, :2], [S], out[:, :, :2])
+
+
+@pytest.mark.parametrize("queries", [3, 40])
+def test_q8_attention_queries_far_apart_and_not_finite(queries):
+    """A query row that is huge, lowest-valued or not finite changes no other row; V near bf16's largest value."""
+    ops = _ops()
+    S = 300
+    c = _held_cache(1, S, 2, 77)
+    c["v_exp"][:, :, 1] = 121
+    q = _randn(6, 1, queries, 2, 128).to(torch.bfloat16)
+    clean = q.clone()
+    q[0, 0] = torch.finfo(torch.bfloat16).min
+    q[0, 1, 0, 5], q[0, 1, 1, 7] = float("inf"), float("nan")
+    d = _cuda(c)
+    args = (d["k"], d["v"], d["k_exp"], d["v_exp"], [S])
+    out, want = (ops.attn_kvcache_q8(t.to(DEV), *args) for t in (q, clean))
+    assert torch.equal(out[:, 2:], want[:, 2:])
+    assert bool(torch.isnan(out[:, 1]).any(-1).all()) and bool(torch.isfinite(want).all())
+    k, v = (ref.values(c[n], c[n + "_exp"]) for n in ("k", "v"))
+    end = torch.full((1, queries), S)
+    exact, weight = ref.span_attention(clean.to(DEV), k.to(DEV), v.to(DEV), torch.zeros_like(end), end)
+    ref.check_attention(want, exact, weight, S)
 
 
 def test_q8_attention_strided_views_scale_and_growing_logits():
