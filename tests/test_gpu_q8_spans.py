@@ -178,6 +178,21 @@ def test_read_back_of_broadcast_rows_into_strided_tensors():
         assert torch.equal(v[b].double().cpu(), ref.values(c["v"][0, s:s + 8], c["v_exp"][0, s:s + 8]))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_read_back_into_tensors_aligned_to_16_bytes_only(dtype):
+    ops = _ops()
+    c = _garbage_cache(2, 30, 3)
+    for n in ("k_exp", "v_exp"):
+        c[n] = c[n].clamp(-126, 121)
+    d = _cuda(c)
+    pad = 128 // torch.finfo(dtype).bits                  # elements in 16 bytes
+    flat = torch.zeros(2 * 2 * 30 * (3 * 128 + pad) + pad, dtype=dtype, device=DEV)
+    out = [flat[pad + i * 30 * 2 * (3 * 128 + pad):].as_strided((2, 30, 3, 128), (30 * (384 + pad), 384 + pad, 128, 1)) for i in range(2)]
+    assert out[0].data_ptr() % 32 == 16
+    k, v = ops.kv_read_q8(d["k"], d["v"], d["k_exp"], d["v_exp"], [0, 0], 30, dtype=dtype, out=out)
+    assert torch.equal(k.double().cpu(), ref.values(c["k"], c["k_exp"])) and torch.equal(v.double().cpu(), ref.values(c["v"], c["v_exp"]))
+
+
 # ------------------------------------------------------------------------------------------------ attention, 8 bits
 def _held_cache(rows, tokens, heads, seed, spread=0.0):
     """A cache that holds unit-variance K and V whose head vectors' scales differ by factors of e^spread."""
