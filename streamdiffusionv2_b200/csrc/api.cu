@@ -557,8 +557,9 @@ static int fill_attn_x(sdv2::AttnXParams& p, int rows, int q_tokens, int heads, 
   p.q_tokens = q_tokens;
   p.heads = heads;
   p.kv_tokens = static_cast<int>(kv_tokens);
+  p.tiles = 2;
   p.pair_tiles = (q_tokens + 255) / 256;
-  if (static_cast<int64_t>(p.pair_tiles) * heads > 0x7FFFFFFFLL / 64 / rows) return SDV2_ERR_UNSUPPORTED_SHAPE;
+  if (2ll * p.pair_tiles * heads > 0x7FFFFFFFLL / 64 / rows) return SDV2_ERR_UNSUPPORTED_SHAPE;
   return SDV2_OK;
 }
 
@@ -588,11 +589,11 @@ static int fill_q_out(sdv2::AttnXParams& p, const sdv2_view* q, const sdv2_view*
 
 static size_t few_bytes(int slots) { return slots * static_cast<size_t>(sdv2::kFewRows) * (128 + 2) * sizeof(float); }
 
-static size_t partial_bytes(int slots) { return slots * sdv2::kAttnXPartFloats * sizeof(float); }
+static size_t partial_bytes(int slots, int tiles) { return slots * tiles * sdv2::kAttnXPartFloats * sizeof(float); }
 
 static void set_partials(sdv2::AttnXParams& p, void* scratch, int slots) {
   p.part_o = slots > 0 ? static_cast<float*>(scratch) : nullptr;
-  p.part_meta = slots > 0 ? p.part_o + static_cast<size_t>(slots) * 2 * 128 * 128 : nullptr;
+  p.part_meta = slots > 0 ? p.part_o + static_cast<size_t>(slots) * p.tiles * 128 * 128 : nullptr;
 }
 
 // How attention over the 8-bit cache runs.  Expanding K/V inside the attention kernel reads each byte once per pair of
@@ -653,7 +654,7 @@ static int plan_q8(Q8Run& r, int heads) {
 size_t sdv2_attn_q8_scratch_bytes(int rows, int q_tokens, int heads, int64_t cache_tokens, const int32_t* seq_lens) {
   Q8Run r;
   if (fill_q8(r, rows, q_tokens, heads, cache_tokens, seq_lens) != SDV2_OK || plan_q8(r, heads) != SDV2_OK) return 0;
-  return 2 * r.expanded + (r.few ? few_bytes(r.slots) : partial_bytes(r.slots));
+  return 2 * r.expanded + (r.few ? few_bytes(r.slots) : partial_bytes(r.slots, r.p.tiles));
 }
 
 int sdv2_attn_kvcache_q8(const sdv2_view* q, const sdv2_view* k_cache, const sdv2_view* v_cache, const sdv2_view* k_exp,
@@ -667,7 +668,7 @@ int sdv2_attn_kvcache_q8(const sdv2_view* q, const sdv2_view* k_cache, const sdv
   if ((rc = fill_q8(r, rows, q_tokens, heads, cache_tokens, seq_lens)) != SDV2_OK) return rc;
   if ((rc = fill_q_out(r.p, q, out, head_dim, softmax_scale, status_dev)) != SDV2_OK) return rc;
   if ((rc = plan_q8(r, heads)) != SDV2_OK) return rc;
-  const size_t need = 2 * r.expanded + (r.few ? few_bytes(r.slots) : partial_bytes(r.slots));
+  const size_t need = 2 * r.expanded + (r.few ? few_bytes(r.slots) : partial_bytes(r.slots, r.p.tiles));
   if (need > 0 && (scratch_dev == nullptr || scratch_bytes < need)) return SDV2_ERR_WORKSPACE;
   if (!aligned16(scratch_dev)) return SDV2_ERR_MISALIGNED;
   char* scratch = static_cast<char*>(scratch_dev);
@@ -734,7 +735,7 @@ size_t sdv2_attn_spans_scratch_bytes(int rows, int q_tokens, int heads, int64_t 
   sdv2::AttnXParams p;
   int slots = 0;
   if (fill_attn_x(p, rows, q_tokens, heads, kv_tokens) != SDV2_OK || plan_spans(p, &slots) != SDV2_OK) return 0;
-  return partial_bytes(slots);
+  return partial_bytes(slots, p.tiles);
 }
 
 int sdv2_attn_spans(const sdv2_view* q, const sdv2_view* k, const sdv2_view* v, const sdv2_view* out, int rows,
@@ -753,7 +754,7 @@ int sdv2_attn_spans(const sdv2_view* q, const sdv2_view* k, const sdv2_view* v, 
   if ((rc = fill_q_out(p, q, out, head_dim, softmax_scale, status_dev)) != SDV2_OK) return rc;
   int slots = 0;
   if ((rc = plan_spans(p, &slots)) != SDV2_OK) return rc;
-  if (slots > 0 && (scratch_dev == nullptr || scratch_bytes < partial_bytes(slots))) return SDV2_ERR_WORKSPACE;
+  if (slots > 0 && (scratch_dev == nullptr || scratch_bytes < partial_bytes(slots, p.tiles))) return SDV2_ERR_WORKSPACE;
   if (!aligned16(scratch_dev)) return SDV2_ERR_MISALIGNED;
   set_partials(p, scratch_dev, slots);
   p.kv_row_broadcast = k->stride_row == 0 ? 1 : 0;

@@ -33,25 +33,39 @@ namespace attnx {
 
 using namespace attn;
 
-constexpr int kRing = 5;
-constexpr int kExpandWarps = 4;
-// Warpgroups: 0 = the issuing warp (and the TMA warp of the span kernel), then with kQ8 one that expands the cache's
-// bytes, then one softmax warpgroup per query tile.  Registers move from the former to the latter: 2 x 176 + 48 + 112 of
-// 4 x 128 a thread at launch, 2 x 200 + 104 of 3 x 168 without the expand warpgroup.
 enum Mode {
   kModeSpans,   // K/V tensors by TMA, a span of keys per query
   kModeExpand,  // 8-bit cache, expanded in the kernel
   kModeLens,    // K/V tensors by TMA, one length per row: the 8-bit cache after kv_read_q8_kernel
 };
 
-template <bool kQ8>
-struct Roles {
-  static constexpr int kSoftmaxWarp0 = kQ8 ? 8 : 4;
-  static constexpr int kThreads = (kSoftmaxWarp0 + 8) * 32;
-  static constexpr int kRegsIssue = kQ8 ? 48 : 104, kRegsExpand = 112, kRegsSoftmax = kQ8 ? 176 : 200;
-  static constexpr int kRegsLaunch = kQ8 ? 128 : 168;
-  static_assert((kQ8 ? kRegsIssue + kRegsExpand : kRegsIssue) + 2 * kRegsSoftmax <= kRegsLaunch * kThreads / 128,
+constexpr int kExpandWarps = 4;
+// Warpgroups: 0 = the issuing warp (and the TMA warp), then with kModeExpand one that expands the cache's bytes, then one
+// softmax warpgroup per query tile.  Registers move from the former to the latter: 2 x 176 + 48 + 112 of 4 x 128 a thread
+// at launch, 2 x 200 + 104 of 3 x 168 without the expand warpgroup, 200 + 56 of 2 x 128 with one query tile.
+//
+// One query tile (kTiles 1) is for short key ranges: 256 TMEM columns and 98 KB let two CTAs share an SM, so that one's
+// set-up, first loads and epilogue pass behind the other's products.  K and V have one slot each there: K_j+1 is loaded
+// while the softmax of tile j runs, V_j+1 while that of tile j+1 does.  Two query tiles share every K/V tile, which long
+// key ranges need: the L2 could not feed two CTAs' own tiles.
+template <int kMode, int kTiles>
+struct Shape {
+  static constexpr bool kExpand = kMode == kModeExpand;
+  static constexpr int kSoftmaxWarp0 = kExpand ? 8 : 4;
+  static constexpr int kThreads = (kSoftmaxWarp0 + 4 * kTiles) * 32;
+  static constexpr int kCtasPerSm = kTiles == 1 ? 2 : 1;
+  static constexpr int kRegsIssue = kExpand ? 48 : kTiles == 1 ? 56 : 104, kRegsExpand = 112;
+  static constexpr int kRegsSoftmax = kExpand ? 176 : 200;
+  static constexpr int kRegsLaunch = kExpand || kTiles == 1 ? 128 : 168;
+  static_assert((kExpand ? kRegsIssue + kRegsExpand : kRegsIssue) + kTiles * kRegsSoftmax <= kRegsLaunch * kThreads / 128,
                 "the warpgroups' shares add up to more than the launch provides");
+  // shared memory: Q tiles | K/V slots | barriers and words | alignment slack
+  static constexpr int kRing = kTiles == 1 ? 2 : 5;
+  static constexpr uint32_t kSmemKV = kTiles * kTileBytes;
+  static constexpr uint32_t kSmemBar = kSmemKV + kRing * kTileBytes;
+  static constexpr uint32_t kSmemBytes = kSmemBar + 256 + 1024;
+  static constexpr uint32_t kTmemCols = 256 * kTiles;
+  static constexpr uint32_t kColS = 0, kColO = 128 * kTiles;
 };
 template <int kRegs>
 __device__ __forceinline__ void regs_dec() {
@@ -61,12 +75,6 @@ template <int kRegs>
 __device__ __forceinline__ void regs_inc() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs));
 }
-constexpr uint32_t kSmemQ = 0;
-constexpr uint32_t kSmemKV = 2 * kTileBytes;
-constexpr uint32_t kSmemBar = kSmemKV + kRing * kTileBytes;
-constexpr uint32_t kSmemBytes = kSmemBar + 256 + 1024;  // + alignment slack
-constexpr uint32_t kTmemCols = 512;
-constexpr uint32_t kColS = 0, kColO = 256;
 
 constexpr int kPairBars = 3;
 constexpr int kBarQFull = 0;                       // [2]
@@ -77,13 +85,15 @@ constexpr int kBarSFull = 3 + 2 * kPairBars;       // [2]
 constexpr int kBarPFull = kBarSFull + 2;           // [2]
 constexpr int kBarOFull = kBarPFull + 2;           // [2]
 constexpr int kBarPHalf = kBarOFull + 2;           // [2] first 64 key columns of P written
-constexpr int kNumBars = kBarPHalf + 2;
-// words behind the barriers: abort flag, TMEM base, hull of the spans, exponents of the last four key tiles
-constexpr uint32_t kSmemWords = kSmemBar + kNumBars * 8;
+constexpr int kBarMask = kBarPHalf + 2;            // the four warps of query tile 0 have noted which keys are attended
+constexpr int kNumBars = kBarMask + 1;
+// with one query tile, by key tile: K in place, V in place, K read, V read
+constexpr int kBarKFull = kBarK0Full, kBarVFull = kBarPairFull, kBarKFree = kBarPairDone, kBarVFree = kBarPairDone + 1;
+// words behind the barriers: abort flag, TMEM base, hull of the spans, exponents of the last four key tiles, keys of a
+// tile that some row attends (three sets of 128 bits in turn)
 constexpr int kWordAbort = 0, kWordTmem = 1, kWordLo = 2, kWordHi = 3, kWordFullLo = 4, kWordFullHi = 5, kWordExpK = 6,
-              kWordExpV = 10, kNumWords = 14;
+              kWordExpV = 10, kWordMask = 14, kNumWords = 26;
 static_assert(kNumBars * 8 + kNumWords * 4 <= 256, "barrier block too small");
-static_assert(kRing >= 5, "pair g overwrites the tiles of pairs g-3 and g-2: needs five slots");
 
 constexpr float kRescaleThreshold = 8.0f;  // log2 units
 
@@ -186,31 +196,43 @@ __device__ __forceinline__ Item find_item(const AttnXParams& p, int i) {
   return it;
 }
 
-template <int kMode>
-__global__ void __launch_bounds__(Roles<kMode == kModeExpand>::kThreads, 1)
+// Bits lo .. hi - 1 of word w of a tile's 128 key bits.
+__device__ __forceinline__ uint32_t span_bits(int lo, int hi, int w) {
+  const int a = max(lo - 32 * w, 0), e = min(hi - 32 * w, 32);
+  if (a >= e) return 0u;
+  return (e == 32 ? 0xFFFFFFFFu : (1u << e) - 1u) & (0xFFFFFFFFu << a);
+}
+
+template <int kMode, int kTiles>
+__global__ void __launch_bounds__(Shape<kMode, kTiles>::kThreads, Shape<kMode, kTiles>::kCtasPerSm)
 attn_x_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
               const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ AttnXParams p) {
   constexpr bool kQ8 = kMode == kModeExpand, kSpans = kMode == kModeSpans;
+  using Sh = Shape<kMode, kTiles>;
+  constexpr int kRing = Sh::kRing;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
   uint8_t* gbase = smem_raw + (base - raw);
-  const uint32_t bar0 = base + kSmemBar;
+  const uint32_t bar0 = base + Sh::kSmemBar;
   auto bar = [&](int i) { return bar0 + 8u * i; };
-  volatile int* words = reinterpret_cast<volatile int*>(gbase + kSmemWords);
+  volatile int* words = reinterpret_cast<volatile int*>(gbase + Sh::kSmemBar + kNumBars * 8);
   volatile int* abort_flag = words + kWordAbort;
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
   const int lane = threadIdx.x & 31;
   const Item item = find_item<kSpans>(p, blockIdx.x);
-  const int b = item.b, h = item.h, q0 = item.tile * (2 * kBM);
-  const bool two_tiles = q0 + kBM < p.q_tokens;
+  const int b = item.b, h = item.h, q0 = item.tile * (kTiles * kBM);
+  const bool two_tiles = kTiles == 2 && q0 + kBM < p.q_tokens;
+  const int n_stage = two_tiles ? 2 : 1;
   const int bk = p.kv_row_broadcast ? 0 : b;
 
   if (threadIdx.x == 0) {
     *abort_flag = 0;
     words[kWordLo] = words[kWordFullHi] = 0x7FFFFFFF;
     words[kWordHi] = words[kWordFullLo] = 0;
+    for (int i = 0; i < 12; ++i) words[kWordMask + i] = 0;
+    mbar_init(bar(kBarMask), 4);
     for (int i = 0; i < 2; ++i) mbar_init(bar(kBarQFull + i), 1);
     mbar_init(bar(kBarK0Full), kQ8 ? kExpandWarps : 1);
     for (int i = 0; i < kPairBars; ++i) {
@@ -224,26 +246,34 @@ attn_x_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
       mbar_init(bar(kBarOFull + i), 1);
     }
     fence_mbar_init();
-    tma_prefetch_desc(&tm_q);
+    for (int s = 0; s < n_stage; ++s) {  // the queries are wanted whatever the keys; the issuing thread waits for them
+      mbar_expect_tx(bar(kBarQFull + s), kTileBytes);
+      tma_load_4d(base + s * kTileBytes, &tm_q, bar(kBarQFull + s), 0, h, q0 + s * kBM, b);
+      tma_load_4d(base + s * kTileBytes + kHalfTile, &tm_q, bar(kBarQFull + s), 64, h, q0 + s * kBM, b);
+    }
     if (!kQ8) {
       tma_prefetch_desc(&tm_k);
       tma_prefetch_desc(&tm_v);
     }
   }
   if (warp == 0) {
-    tmem_alloc(smem_u32(const_cast<int*>(words + kWordTmem)), kTmemCols);
+    tmem_alloc(smem_u32(const_cast<int*>(words + kWordTmem)), Sh::kTmemCols);
     tmem_relinquish();
   }
-  // this thread's query row (softmax warps) and its span, clipped to the keys there are
-  int span_lo = 0, span_hi = 0;
-  constexpr int kSoftmaxWarp0 = Roles<kQ8>::kSoftmaxWarp0;
-  const int my_row = q0 + (warp - kSoftmaxWarp0) * 32 + lane;  // eight warps for the 256 rows of the tile pair
-  if (kSpans && warp >= kSoftmaxWarp0 && my_row < p.q_tokens) {
-    const int64_t at = b * p.end_stride_row + static_cast<int64_t>(my_row) * p.end_stride_tok;
-    span_hi = min(p.end[at], p.kv_tokens);
-    if (p.begin != nullptr)
-      span_lo = max(p.begin[b * p.begin_stride_row + static_cast<int64_t>(my_row) * p.begin_stride_tok], 0);
-    if (span_lo >= span_hi) span_lo = span_hi = 0;
+  // this thread's query row (softmax warps) and its span, clipped to the keys there are; for the threads of query tile 0
+  // that of the row 128 further on too
+  constexpr int kSoftmaxWarp0 = Sh::kSoftmaxWarp0;
+  const int my_row = q0 + (warp - kSoftmaxWarp0) * 32 + lane;  // four warps for the 128 rows of a query tile
+  int span_lo = 0, span_hi = 0, span2_lo = 0, span2_hi = 0;
+  auto load_span = [&](int row, int& lo, int& hi) {
+    if (row >= p.q_tokens) return;
+    hi = min(p.end[b * p.end_stride_row + static_cast<int64_t>(row) * p.end_stride_tok], p.kv_tokens);
+    lo = p.begin == nullptr ? 0 : max(p.begin[b * p.begin_stride_row + static_cast<int64_t>(row) * p.begin_stride_tok], 0);
+    if (lo >= hi) lo = hi = 0;
+  };
+  if (kSpans && warp >= kSoftmaxWarp0) {
+    load_span(my_row, span_lo, span_hi);
+    if (kTiles == 2 && warp < kSoftmaxWarp0 + 4) load_span(my_row + kBM, span2_lo, span2_hi);
   }
   tc_fence_before();
   __syncthreads();
@@ -272,35 +302,56 @@ attn_x_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
                                           : static_cast<int>(static_cast<int64_t>(item.part + 1) * n_kv_all / item.parts));
   const int n_kv = j1 - j0;  // may be 0: nothing to attend
 
-  auto slot_off = [&](int it) { return kSmemKV + (it % kRing) * kTileBytes; };
+  auto slot_off = [&](int it) { return Sh::kSmemKV + (it % kRing) * kTileBytes; };
 
-  if (warp < 4) regs_dec<Roles<kQ8>::kRegsIssue>();
+  if (warp < 4) regs_dec<Sh::kRegsIssue>();
   if (warp == 0) {
     // ------------------------------------------------------------------ MMA issuer
-    if (lane == 0 && n_kv > 0) {
-      const int n_stage = two_tiles ? 2 : 1;
-      for (int s = 0; s < n_stage; ++s) {
-        mbar_expect_tx(bar(kBarQFull + s), kTileBytes);
-        tma_load_4d(base + kSmemQ + s * kTileBytes, &tm_q, bar(kBarQFull + s), 0, h, q0 + s * kBM, b);
-        tma_load_4d(base + kSmemQ + s * kTileBytes + kHalfTile, &tm_q, bar(kBarQFull + s), 64, h, q0 + s * kBM, b);
-      }
-      const uint32_t sq[2] = {base + kSmemQ, base + kSmemQ + kTileBytes};
-      const uint32_t tS[2] = {tmem + kColS, tmem + kColS + 128};
-      const uint32_t tO[2] = {tmem + kColO, tmem + kColO + 128};
-      // Q first and unconditionally: this thread must not leave while its copies are in flight
+    if (lane == 0) {
+      const uint32_t sq[2] = {base, base + kTileBytes};
+      const uint32_t tS[2] = {tmem + Sh::kColS, tmem + Sh::kColS + 128};
+      const uint32_t tO[2] = {tmem + Sh::kColO, tmem + Sh::kColO + 128};
+      // without condition: this thread must not leave while its copies are in flight
       bool ok = true;
       for (int s = 0; s < n_stage; ++s) ok = mbar_wait(bar(kBarQFull + s), 0, abort_flag, p.status, WAIT_Q_FULL) && ok;
-      ok = ok && mbar_wait(bar(kBarK0Full), 0, abort_flag, p.status, WAIT_KV_FULL);
+      ok = ok && n_kv > 0 && mbar_wait(bar(kBarK0Full), 0, abort_flag, p.status, WAIT_KV_FULL);
       for (int s = 0; s < n_stage && ok; ++s) {
         tc_fence_after();
         issue_qk(tS[s], sq[s], base + slot_off(0));
         umma_commit(bar(kBarSFull + s));
       }
+      if (kTiles == 1) {
+        if (ok) umma_commit(bar(kBarKFree));
+        for (int j = 0; j < n_kv && ok; ++j) {
+          const uint32_t sk = base + slot_off(0), sv = base + slot_off(1);
+          ok = mbar_wait(bar(kBarPHalf), j & 1, abort_flag, p.status, WAIT_P_FULL) &&
+               mbar_wait(bar(kBarVFull), j & 1, abort_flag, p.status, WAIT_KV_FULL);
+          if (!ok) break;
+          tc_fence_after();
+          issue_pv(tO[0], tS[0], sv, j > 0, 0, 4);
+          ok = mbar_wait(bar(kBarPFull), j & 1, abort_flag, p.status, WAIT_P_FULL);
+          if (!ok) break;
+          tc_fence_after();
+          issue_pv(tO[0], tS[0], sv, true, 4, 8);
+          umma_commit(bar(kBarVFree));
+          if (j + 1 < n_kv) {
+            ok = mbar_wait(bar(kBarKFull), (j + 1) & 1, abort_flag, p.status, WAIT_KV_FULL);
+            if (!ok) break;
+            tc_fence_after();
+            issue_qk(tS[0], sq[0], sk);
+            umma_commit(bar(kBarSFull));
+            umma_commit(bar(kBarKFree));
+          } else {
+            umma_commit(bar(kBarOFull));
+          }
+        }
+        ok = false;  // done; the loop below is that of two query tiles
+      }
       // step j: O += P_j V_j and S = Q K_{j+1}^T for each query tile; V_j and K_{j+1} are pair j of the ring
       int slot_v = 1 % kRing, slot_k = 2 % kRing, pair_bar = 0, pair_par = 0;
-      for (int j = 0; j < n_kv && ok; ++j) {
+      for (int j = 0; kTiles == 2 && j < n_kv && ok; ++j) {
         const bool more = j + 1 < n_kv;
-        const uint32_t sv = base + kSmemKV + slot_v * kTileBytes, sk = base + kSmemKV + slot_k * kTileBytes;
+        const uint32_t sv = base + Sh::kSmemKV + slot_v * kTileBytes, sk = base + Sh::kSmemKV + slot_k * kTileBytes;
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
           if (s >= n_stage || !ok) break;
@@ -336,7 +387,7 @@ attn_x_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
   } else if (warp < kSoftmaxWarp0) {
     if (kQ8 && warp >= 4) {
       // ---------------------------------------------------------------- expand warps
-      regs_dec<Roles<kQ8>::kRegsExpand>();
+      regs_dec<Sh::kRegsExpand>();
       const int w = warp - 4;
       const int tok = j0 * kBN + w * 4 + lane_token(lane);
       const uint8_t* kb = static_cast<const uint8_t*>(p.k.ptr) + bk * p.k.stride_row + h * p.k.stride_head + lane_byte(lane);
@@ -400,8 +451,36 @@ attn_x_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
       mbar_expect_tx(bar(kBarK0Full), kTileBytes);
       load_tile(&tm_k, 0, 0, bar(kBarK0Full));
       bool ok = true;
+      if (kTiles == 1) {
+        int g = 0;
+        bool k_ahead = false;  // the K load of tile g was made
+        for (; g < n_kv; ++g) {
+          k_ahead = g == 0;
+          if (g > 0) {
+            ok = mbar_wait(bar(kBarKFree), (g - 1) & 1, abort_flag, p.status, WAIT_KV_EMPTY);
+            if (!ok) break;
+            mbar_expect_tx(bar(kBarKFull), kTileBytes);
+            load_tile(&tm_k, 0, g, bar(kBarKFull));
+            k_ahead = true;
+            ok = mbar_wait(bar(kBarVFree), (g - 1) & 1, abort_flag, p.status, WAIT_KV_EMPTY);
+            if (!ok) break;
+          }
+          mbar_expect_tx(bar(kBarVFull), kTileBytes);
+          load_tile(&tm_v, 1, g, bar(kBarVFull));
+        }
+        if (!ok) {  // leave no copy in flight: the last of either kind (an earlier one has been consumed)
+          const long long t0 = clock64();
+          const int last_k = k_ahead ? g : g - 1;
+          while (!mbar_try_wait(bar(kBarKFull), last_k & 1) && clock64() - t0 < kWaitBudgetCycles) {
+          }
+          const long long t1 = clock64();
+          while (g > 0 && !mbar_try_wait(bar(kBarVFull), (g - 1) & 1) && clock64() - t1 < kWaitBudgetCycles) {
+          }
+        }
+        ok = true;  // done; the rest is for two query tiles
+      }
       int issued = 0;  // pairs requested
-      for (int g = 0; g < n_kv; ++g) {
+      for (int g = 0; kTiles == 2 && g < n_kv; ++g) {
         if (g >= 2)
           ok = mbar_wait(bar(kBarPairDone + (g - 2) % kPairBars), ((g - 2) / kPairBars) & 1, abort_flag, p.status,
                          WAIT_KV_EMPTY);
@@ -428,19 +507,20 @@ attn_x_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
     }
   } else {
     // ------------------------------------------------------------------ softmax + epilogue
-    regs_inc<Roles<kQ8>::kRegsSoftmax>();
+    regs_inc<Sh::kRegsSoftmax>();
     const int stage = (warp - kSoftmaxWarp0) >> 2;
     if (stage == 0 || two_tiles) {
       const int quad = warp & 3;
       const int row = quad * 32 + lane;
       const uint32_t lane_base = static_cast<uint32_t>(quad * 32) << 16;
-      const uint32_t tS = tmem + lane_base + kColS + stage * 128;
-      const uint32_t tO = tmem + lane_base + kColO + stage * 128;
+      const uint32_t tS = tmem + lane_base + Sh::kColS + stage * 128;
+      const uint32_t tO = tmem + lane_base + Sh::kColO + stage * 128;
       const int full_lo = kSpans ? words[kWordFullLo] : 0, full_hi = kSpans ? words[kWordFullHi] : key_hi;
       float m_used = -INFINITY;  // running maximum (lags by up to the threshold); -inf: no key so far
       float l = 0.f;
       int ref_v = 0;  // V exponent the accumulator is in (kQ8)
       bool ok = true;
+      int n_mixed = 0;
       for (int j = 0; j < n_kv; ++j) {
         const int key0 = (j0 + j) * kBN;
         // V rows that no query row of this CTA attends lie inside the tensor, so the TMA did not zero-fill them and they
@@ -448,21 +528,34 @@ attn_x_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
         // them in shared memory before it reports P (tile 1's P V is issued later), and before it holds a tile of S in
         // registers.  (kQ8: expanded as zeros.)
         if (!kQ8 && stage == 0 && (key0 < full_lo || key0 + kBN > full_hi)) {
-          ok = mbar_wait(bar(kBarPairFull + j % kPairBars), (j / kPairBars) & 1, abort_flag, p.status, WAIT_KV_FULL);
+          // which keys some row attends: each warp adds its rows' (and those 128 further on) to the tile's 128 bits
+          bool attended = key0 + row < key_hi;  // kModeLens: one length for all
+          if (kSpans) {
+            volatile int* bits = words + kWordMask + (n_mixed % 3) * 4;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              uint32_t mine = span_bits(span_lo - key0, span_hi - key0, w);
+              if (kTiles == 2) mine |= span_bits(span2_lo - key0, span2_hi - key0, w);
+              mine = __reduce_or_sync(0xffffffffu, mine);
+              if (lane == w) {
+                atomicOr(const_cast<int*>(bits + w), static_cast<int>(mine));
+                // the set of the next mixed tile: everyone has read what it held two tiles ago
+                if (quad == 0) words[kWordMask + ((n_mixed + 1) % 3) * 4 + w] = 0;
+              }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(kBarMask));
+            ok = mbar_wait(bar(kBarMask), n_mixed & 1, abort_flag, p.status, WAIT_MASK);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            attended = (static_cast<uint32_t>(bits[row >> 5]) >> (row & 31)) & 1u;
+            ++n_mixed;
+          }
+          ok = kTiles == 1 ? mbar_wait(bar(kBarVFull), j & 1, abort_flag, p.status, WAIT_KV_FULL)
+                           : mbar_wait(bar(kBarPairFull + j % kPairBars), (j / kPairBars) & 1, abort_flag, p.status, WAIT_KV_FULL);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
-          const int key = key0 + row;
-          const bool in_hull = key >= key_lo && key < key_hi;
-          bool attended = !kSpans;  // one length per row: every row attends the whole hull
-          // rows in a scattered order, so that a few of them usually settle it
-          for (int i = 0; i < 2 * kBM && __any_sync(0xffffffffu, in_hull && !attended); ++i) {
-            const int r = q0 + ((i * 97) & (2 * kBM - 1));
-            if (r >= p.q_tokens) continue;
-            const int e = p.end[b * p.end_stride_row + static_cast<int64_t>(r) * p.end_stride_tok];
-            const int a = p.begin == nullptr ? 0 : p.begin[b * p.begin_stride_row + static_cast<int64_t>(r) * p.begin_stride_tok];
-            attended = attended || (key >= a && key < e);
-          }
-          if (!(in_hull && attended)) {
+          if (!attended) {
             uint8_t* vrow = gbase + slot_off(2 * j + 1) + row * 128;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
@@ -599,8 +692,8 @@ attn_x_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
         }
       } else if (ok) {
         // partial result of one key range: unnormalised accumulator, running maximum and sum, V exponent
-        float* po = p.part_o + (static_cast<size_t>(item.slot) * 2 + stage) * (kBM * kHD) + row * kHD;
-        float* pm = p.part_meta + (static_cast<size_t>(item.slot) * 2 + stage) * (3 * kBM);
+        float* po = p.part_o + (static_cast<size_t>(item.slot) * kTiles + stage) * (kBM * kHD) + row * kHD;
+        float* pm = p.part_meta + (static_cast<size_t>(item.slot) * kTiles + stage) * (3 * kBM);
         pm[row] = m_used;
         pm[kBM + row] = l;
         pm[2 * kBM + row] = static_cast<float>(ref_v);
@@ -624,14 +717,14 @@ attn_x_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
   __syncthreads();
   if (warp == 0) {
     tc_fence_after();
-    tmem_dealloc(tmem, kTmemCols);
+    tmem_dealloc(tmem, Sh::kTmemCols);
   }
 }
 
 // Merge the parts of the split tiles.  Block = (split tile, query tile, group of 32 rows); 256 threads = 32 rows x 8
 // column groups of 16.  out = sum_k w_k O_k / sum_k 2^(m_k - m) l_k with w_k = 2^(m_k - m + R_k - R) and the result in
 // units of 2^(R+6); a part without a key has l_k = 0 and no accumulator.
-template <int kMode>
+template <int kMode, int kTiles>
 __global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ AttnXParams p) {
   constexpr bool kQ8 = kMode == kModeExpand, kSpans = kMode == kModeSpans;
   const int stage = blockIdx.y;
@@ -639,11 +732,11 @@ __global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ At
   const int c0 = (threadIdx.x & 7) * 16;
   const Item item =
       find_item<kSpans>(p, kSpans ? p.n_full + static_cast<int>(blockIdx.x) * p.split : first_item_lens(p, blockIdx.x));
-  const int q_row = item.tile * (2 * kBM) + stage * kBM + row;
+  const int q_row = item.tile * (kTiles * kBM) + stage * kBM + row;
   if (item.part < 0 || q_row >= p.q_tokens) return;
-  const float* pm = p.part_meta + (static_cast<size_t>(item.slot) * 2 + stage) * (3 * kBM) + row;
-  const float* po = p.part_o + (static_cast<size_t>(item.slot) * 2 + stage) * (kBM * kHD) + row * kHD + c0;
-  constexpr size_t pm_step = 2 * 3 * kBM, po_step = static_cast<size_t>(2) * kBM * kHD;
+  const float* pm = p.part_meta + (static_cast<size_t>(item.slot) * kTiles + stage) * (3 * kBM) + row;
+  const float* po = p.part_o + (static_cast<size_t>(item.slot) * kTiles + stage) * (kBM * kHD) + row * kHD + c0;
+  constexpr size_t pm_step = kTiles * 3 * kBM, po_step = static_cast<size_t>(kTiles) * kBM * kHD;
   float m = -INFINITY, ref = q8::kMinExp;
   for (int k = 0; k < item.parts; ++k) {
     m = fmaxf(m, pm[k * pm_step]);
@@ -680,50 +773,56 @@ __global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ At
                    pack_bf16x2(acc[8 * i + 4], acc[8 * i + 5]), pack_bf16x2(acc[8 * i + 6], acc[8 * i + 7]));
 }
 
-template <int kMode>
+template <int kMode, int kTiles>
 cudaError_t launch(const CUtensorMap& tm_q, const CUtensorMap& tm_k, const CUtensorMap& tm_v, const AttnXParams& p,
                    cudaStream_t stream) {
   constexpr bool kSpans = kMode == kModeSpans;
   static DynamicSmemGrant smem_grant;  // one per instantiation
   DeviceInfo di;
   cudaError_t e = device_info(&di);
-  if (e == cudaSuccess) e = smem_grant.ensure(attn_x_kernel<kMode>, static_cast<int>(kSmemBytes), di.device);
+  if (e == cudaSuccess) e = smem_grant.ensure(attn_x_kernel<kMode, kTiles>, static_cast<int>(Shape<kMode, kTiles>::kSmemBytes), di.device);
   if (e != cudaSuccess) return e;
   const int items = p.n_full + p.n_parts;
-  attn_x_kernel<kMode><<<items, Roles<kMode == kModeExpand>::kThreads, kSmemBytes, stream>>>(tm_q, tm_k, tm_v, p);
+  attn_x_kernel<kMode, kTiles><<<items, Shape<kMode, kTiles>::kThreads, Shape<kMode, kTiles>::kSmemBytes, stream>>>(
+      tm_q, tm_k, tm_v, p);
   e = cudaGetLastError();
   if (e != cudaSuccess || p.split == 1) return e;
   const int merged = p.n_tiles - p.n_full;
-  combine_kernel<kMode><<<dim3(merged, p.q_tokens > kBM ? 2 : 1, kBM / 32), 256, 0, stream>>>(p);
+  combine_kernel<kMode, kTiles><<<dim3(merged, kTiles == 2 && p.q_tokens > kBM ? 2 : 1, kBM / 32), 256, 0, stream>>>(p);
   return cudaGetLastError();
 }
 
 }  // namespace attnx
 
 cudaError_t launch_attn_q8_expand(const CUtensorMap& tm_q, const AttnXParams& p, cudaStream_t stream) {
-  return attnx::launch<attnx::kModeExpand>(tm_q, tm_q, tm_q, p, stream);
+  return attnx::launch<attnx::kModeExpand, 2>(tm_q, tm_q, tm_q, p, stream);
 }
 
 cudaError_t launch_attn_lens(const CUtensorMap& tm_q, const CUtensorMap& tm_k, const CUtensorMap& tm_v,
                              const AttnXParams& p, cudaStream_t stream) {
-  return attnx::launch<attnx::kModeLens>(tm_q, tm_k, tm_v, p, stream);
+  return attnx::launch<attnx::kModeLens, 2>(tm_q, tm_k, tm_v, p, stream);
 }
 
 cudaError_t launch_attn_spans(const CUtensorMap& tm_q, const CUtensorMap& tm_k, const CUtensorMap& tm_v,
                               const AttnXParams& p, cudaStream_t stream) {
-  return attnx::launch<attnx::kModeSpans>(tm_q, tm_k, tm_v, p, stream);
+  return p.tiles == 1 ? attnx::launch<attnx::kModeSpans, 1>(tm_q, tm_k, tm_v, p, stream)
+                      : attnx::launch<attnx::kModeSpans, 2>(tm_q, tm_k, tm_v, p, stream);
 }
 
 // Spans live on the device, so the host cuts the tail's tiles by their number and the number of keys alone; a part whose
 // share is empty costs little.  Tiles before the tail run late queries first.
 int plan_spans(AttnXParams& p, int sms) {
   constexpr int kMinTiles = 4;
+  constexpr int kShortKeys = 1024;
+  p.tiles = p.kv_tokens <= kShortKeys || p.q_tokens <= 128 ? 1 : 2;
+  p.pair_tiles = (p.q_tokens + 128 * p.tiles - 1) / (128 * p.tiles);
+  const int wave = p.tiles == 1 ? 2 * sms : sms;
   const int64_t n_tiles = static_cast<int64_t>(p.pair_tiles) * p.heads * p.rows;
   if (n_tiles > 0x7FFFFFFFLL / 64) return -1;
   p.n_tiles = static_cast<int>(n_tiles);
-  const int tail = p.n_tiles % sms;
+  const int tail = p.n_tiles % wave;
   p.n_full = p.n_tiles - tail;
-  p.split = tail == 0 ? 1 : max(1, min(min(sms / tail, 64), (p.kv_tokens + 127) / 128 / kMinTiles));
+  p.split = tail == 0 ? 1 : max(1, min(min(wave / tail, 64), (p.kv_tokens + 127) / 128 / kMinTiles));
   p.n_parts = tail * p.split;
   return p.split > 1 ? p.n_parts : 0;
 }

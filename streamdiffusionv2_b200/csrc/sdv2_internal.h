@@ -195,9 +195,10 @@ struct AttnXParams {
   int kv_row_broadcast;  // 1: every row reads K/V row 0
   float scale_log2;      // softmax_scale * log2(e)
   int* status;
-  float* part_o;         // [parts][2][128][128] fp32
-  float* part_meta;      // [parts][2][3][128] fp32: running maximum (log2 units), sum, V exponent
-  int pair_tiles, n_tiles;
+  float* part_o;         // [parts][tiles][128][128] fp32
+  float* part_meta;      // [parts][tiles][3][128] fp32: running maximum (log2 units), sum, V exponent
+  int tiles;             // 128-row query tiles that a CTA has (spans: 1 or 2, else 2)
+  int pair_tiles, n_tiles;  // CTAs' worth of query rows per (head, row); of them in all
   int n_full, n_parts;   // tiles [0, n_full) run whole, the others in parts, n_parts of them in all
   int split;             // spans: parts of each of the others; lengths: the most parts of one of them
   // 8-bit cache, lengths: rows longest first, parts[r] parts for the tiles of a row
@@ -211,7 +212,7 @@ struct AttnXParams {
   const int* end;
   int64_t begin_stride_row, begin_stride_tok, end_stride_row, end_stride_tok;
 };
-constexpr size_t kAttnXPartFloats = 2 * (128 * 128 + 3 * 128);
+constexpr size_t kAttnXPartFloats = 128 * 128 + 3 * 128;  // of one query tile
 // Fill in how the work is cut up; returns the partial-result slots needed (0: none) or -1 (too many tiles).
 int plan_lens(AttnXParams& p, int wave, int min_tiles);
 int plan_spans(AttnXParams& p, int sms);
