@@ -353,7 +353,7 @@ size_t sdv2_attn_q8_scratch_bytes(int rows, int q_tokens, int heads, int64_t cac
  * (begin 0, end the length), block-causal clips (end the end of the query's block), packed clips (begin and end of the
  * query's own), windows.  Spans are clipped to [0, kv_tokens); a query whose span is empty gets 0.
  * Covers WanT2VCrossAttention.forward with context_lens (models/wan/wan_base/modules/model.py:161-194) and the masks of
- * CausalWanSelfAttention.forward without a cache (models/wan/causal_model.py:219-248).
+ * CausalWanSelfAttention.forward without a cache (models/wan/causal_model.py:220-249).
  *
  * bf16 in and out, fp32 accumulate, head_dim 128; k / v stride_row may be 0.  begin_dev (NULL: 0) and end_dev: device
  * int32, element strides per row and per query, 0 allowed (one span for all); read when the kernel runs.

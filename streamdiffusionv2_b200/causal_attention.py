@@ -17,7 +17,7 @@ from __future__ import annotations
 import inspect
 import math
 import types
-from typing import List, Optional, Sequence
+from typing import List, NamedTuple, Optional, Sequence
 
 import torch
 
@@ -82,8 +82,12 @@ def adaptive_similarities(kv_cache, roped_k, v, sink_size: int, frame_tokens: in
     device: the threshold test and everything that follows from it run in the plan kernel."""
     rows = roped_k.shape[0]
     if roped_k.is_cuda:
-        # the four means in two launches, straight from the cache (no reshaped copies)
-        means = ops.frame_means(kv_cache["k"][:rows], kv_cache["v"][:rows], roped_k, v, sink_size, frame_tokens)
+        # the four means in two launches, straight from the cache (no reshaped copies; an 8-bit cache's sink is read back)
+        k_cache, v_cache = kv_cache["k"][:rows], kv_cache["v"][:rows]
+        if "k_exp" in kv_cache:
+            k_cache, v_cache = ops.kv_read_q8(k_cache, v_cache, kv_cache["k_exp"][:rows], kv_cache["v_exp"][:rows],
+                                              [0] * rows, sink_size * frame_tokens, dtype=roped_k.dtype)
+        means = ops.frame_means(k_cache, v_cache, roped_k, v, sink_size, frame_tokens)
         k_sink, k_new = means[:, :sink_size, 0], means[:, sink_size:, 0]
         v_sink, v_new = means[:, :sink_size, 1], means[:, sink_size:, 1]
     else:                                      # host tensors: only the tests of the host logic come here
@@ -101,6 +105,43 @@ def sync_evict_queue(attn_module) -> None:
     """Refresh `attn_module.evict_idx` (the reference's attribute) from the device-resident queue that
     the adaptive sink path keeps (one read-back); no-op for modules whose queue lives on the host."""
     RingState.sync_queue(attn_module)
+
+
+def cache_tensors(kv_cache) -> tuple:
+    """Names of a cache dict's per-token tensors: "k", "v" and, for an 8-bit cache (`ops.q8_cache`), "k_exp", "v_exp"."""
+    return ("k", "v", "k_exp", "v_exp") if "k_exp" in kv_cache else ("k", "v")
+
+
+class KeySpans(NamedTuple):
+    """Which keys every query attends, for attention without a cache: begin (None: 0) and end, int32 [B, N] on the device
+    (any strides).  Passed where the reference passes its block mask."""
+    begin: Optional[torch.Tensor]
+    end: torch.Tensor
+
+
+def block_causal_spans(frames: int, frame_tokens: int, frames_per_block: int, device, rows: int = 1,
+                       window_frames: int = -1) -> KeySpans:
+    """Spans of a clip processed in one pass: a token attends its own block of frames and every block before it
+    (the training branch's mask, models/wan/causal_model.py:220-249), with window_frames > 0 only from window_frames frames before its block's end."""
+    t = torch.arange(frames * frame_tokens, device=device)
+    block = frames_per_block * frame_tokens
+    end = ((t // block + 1) * block).clamp_max(frames * frame_tokens)
+    begin = None if window_frames <= 0 else (end - window_frames * frame_tokens).clamp_min(0).int().expand(rows, -1)
+    return KeySpans(begin, end.int().expand(rows, -1))
+
+
+def clip_attention(q, k, v, grid_sizes, freqs, spans: KeySpans, norm=None):
+    """Rope and attention of a whole clip without a cache: already projected q/k/v [B, N, H, D] in bf16, `norm` as for
+    `cached_attention`.  Inference only (no gradient is recorded)."""
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v)):
+        raise RuntimeError("attention over key spans records no gradient: call it under torch.no_grad()")
+    B, n, H, D = q.shape
+    grid = tuple(int(x) for x in grid_sizes[0].tolist())
+    table = ops.rope_table_device(freqs, q.device)
+    rk = torch.empty((B, n, H, D), dtype=k.dtype, device=k.device)
+    rv = torch.empty_like(rk)
+    rq = ops.rope_kv_append(q, k, v, rk, rv, table, grid, [0] * B, [0] * B, **({} if norm is None else {"norm": norm}))
+    return ops.attn_spans(rq, rk, rv, spans.begin, spans.end)
 
 
 def cached_attention(attn_module, q, k, v, grid_sizes, freqs, kv_cache, current_start, norm=None):
@@ -122,6 +163,20 @@ def cached_attention(attn_module, q, k, v, grid_sizes, freqs, kv_cache, current_
     index_tensors = (kv_cache["global_end_index"], kv_cache["local_end_index"])
     sink_tokens = attn_module.sink_size * frame_tokens
     adaptive = sink_tokens > 0 and attn_module.adapt_sink_thr > -1 and n_new <= frame_tokens
+    q8 = "k_exp" in kv_cache
+    if q8 and norm is not None:          # the 8-bit append takes normalised q and k
+        q, k = (ops.rmsnorm(t.flatten(2), w, norm[2]).view(B, n_new, H, D) for t, w in ((q, norm[0]), (k, norm[1])))
+        norm = None
+
+    if q8:
+        held = [kv_cache[name][:B] for name in ("k", "v", "k_exp", "v_exp")]
+
+    def append(slots, **kw):
+        if q8:
+            return ops.rope_kv_append_q8(q, k, v, *held, table, (f, gh, gw), start_frames, slots,
+                                         index_tensors=index_tensors, **kw)
+        return ops.rope_kv_append(q, k, v, kv_cache["k"], kv_cache["v"], table, (f, gh, gw), start_frames, slots,
+                                  index_tensors=index_tensors, **kw)
 
     extra = {} if norm is None else {"norm": norm}
     if not adaptive:
@@ -129,9 +184,7 @@ def cached_attention(attn_module, q, k, v, grid_sizes, freqs, kv_cache, current_
         if _step_recorder is not None:
             extra["step_params"] = _step_recorder.layer_params(attn_module, kv_cache, start_frames, dst, state,
                                                                seq_lens, n_new, frame_tokens)
-        roped_q = ops.rope_kv_append(q, k, v, kv_cache["k"], kv_cache["v"], table, (f, gh, gw), start_frames,
-                                     dst, index_tensors=index_tensors,
-                                     index_values=(state.global_end, state.local_end), **extra)
+        roped_q = append(dst, index_values=(state.global_end, state.local_end), **extra)
     else:
         # The slot of a row depends on the data (roped k against the sink frames already in the cache), so the
         # queue lives on the device: rope into a staging chunk, compute the similarities there, let the plan
@@ -161,10 +214,11 @@ def cached_attention(attn_module, q, k, v, grid_sizes, freqs, kv_cache, current_
         ops.rope_kv_append(q, k, v, stage_k, stage_v, table, (f, gh, gw), start_frames, [0] * B, **stage_kw)
         sim = adaptive_similarities(kv_cache, stage_k, stage_v, attn_module.sink_size, frame_tokens)
         ops.ring_plan_adaptive(sim, attn_module.adapt_sink_thr, queue, frame_tokens, n_new, step_params, **plan_kw)
-        roped_q = ops.rope_kv_append(q, k, v, kv_cache["k"], kv_cache["v"], table, (f, gh, gw), start_frames,
-                                     [0] * B, index_tensors=index_tensors, step_params=step_params, **extra)
+        roped_q = append([0] * B, step_params=step_params, **extra)
 
-    if q.dtype == torch.bfloat16:
+    if q8:
+        out = ops.attn_kvcache_q8(roped_q, *held, seq_lens)
+    elif q.dtype == torch.bfloat16:
         out = ops.attn_kvcache(roped_q, kv_cache["k"], kv_cache["v"], seq_lens)
     else:
         out = ops.attn_kvcache_simt(roped_q, kv_cache["k"], kv_cache["v"], seq_lens)
@@ -242,8 +296,12 @@ def project_qkv(attn, x):
 
 def self_attention_forward(self, x, seq_lens, grid_sizes, freqs, block_mask, kv_cache=None, current_start=0,
                            current_end=0, causal_rope_cache=None):
-    """Drop-in for CausalWanSelfAttention.forward on the kv-cache path (the training branch, which
-    the streaming pipelines never take, is delegated to the original forward)."""
+    """Drop-in for CausalWanSelfAttention.forward on the kv-cache path.  Without a cache a `KeySpans` in the block
+    mask's place runs the clip in one pass; any other mask (the training branch, which the streaming pipelines never
+    take) is delegated to the original forward."""
+    if kv_cache is None and isinstance(block_mask, KeySpans):
+        q, k, v, norm = project_qkv(self, x)
+        return self.o(clip_attention(q, k, v, grid_sizes, freqs, block_mask, norm=norm).flatten(2))
     if kv_cache is None:
         original = getattr(self, "_sdv2_original_forward", None)
         if original is None:
@@ -256,7 +314,8 @@ def self_attention_forward(self, x, seq_lens, grid_sizes, freqs, block_mask, kv_
 
 def cross_attention_forward(self, x, context, context_lens, crossattn_cache=None):
     """Drop-in for WanT2VCrossAttention.forward: K/V of the text context are computed on the
-    first call after `is_init` was cleared and read from the cache afterwards."""
+    first call after `is_init` was cleared and read from the cache afterwards.  `context_lens` (one per row: a tensor
+    or ints), where given, keeps a row's queries to its first context_lens tokens; a row of length 0 gets 0."""
     b, n, d = x.size(0), self.num_heads, self.head_dim
     q = _qk_norm(self.norm_q, self.q(x)).view(b, -1, n, d)
     if crossattn_cache is not None:
@@ -273,8 +332,13 @@ def cross_attention_forward(self, x, context, context_lens, crossattn_cache=None
         k = self.norm_k(self.k(context)).view(b, -1, n, d)
         v = self.v(context).view(b, -1, n, d)
     if context_lens is not None:
-        raise NotImplementedError("per-sample context lengths are not used on the streaming path")
-    if q.dtype == torch.bfloat16:
+        if q.dtype != torch.bfloat16:
+            raise NotImplementedError("per-sample context lengths need bf16 tensors")
+        if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v)):
+            raise RuntimeError("attention with context lengths records no gradient: call it under torch.no_grad()")
+        lens = torch.as_tensor(context_lens, dtype=torch.int32, device=q.device).reshape(b, 1)
+        out = ops.attn_spans(q, k, v, None, lens.expand(b, q.shape[1]))
+    elif q.dtype == torch.bfloat16:
         out = ops.cross_attn(q, k, v)
     else:
         out = ops.attn_kvcache_simt(q, k, v, [k.shape[1]] * b)

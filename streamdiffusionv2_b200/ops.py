@@ -390,13 +390,16 @@ def _cuda_device(what: str, t: torch.Tensor) -> torch.device:
     return t.device
 
 
+Q8_MIN_EXP = -126          # smallest exponent of the 8-bit cache format: that of a vector of zeros
+
+
 def q8_cache(rows: int, tokens: int, heads: int, device) -> Dict[str, torch.Tensor]:
     """The four tensors of an 8-bit K/V cache, holding zeros: "k", "v" uint8 [rows, tokens, heads, 128] and "k_exp",
     "v_exp" int8 [rows, tokens, heads].  A head vector holds sign * magnitude * 2^exponent, the sign in a byte's top
     bit; see `rope_kv_append_q8`."""
     shape = (rows, tokens, heads, 128)
     out = {n: torch.zeros(shape, dtype=torch.uint8, device=device) for n in ("k", "v")}
-    out.update({n: torch.zeros(shape[:3], dtype=torch.int8, device=device) for n in ("k_exp", "v_exp")})
+    out.update({n: torch.full(shape[:3], Q8_MIN_EXP, dtype=torch.int8, device=device) for n in ("k_exp", "v_exp")})
     return out
 
 

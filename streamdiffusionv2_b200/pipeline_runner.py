@@ -20,6 +20,8 @@ from typing import List, Optional, Sequence
 
 import torch
 
+from . import ops
+from .causal_attention import cache_tensors
 from .ring_state import RingState
 from .stage_transport import StageLink, StagePacket, contiguous_block_ranges, plan_from_measurements
 from .stream_pipeline import StreamPipeline, assign_ints
@@ -300,10 +302,10 @@ class PipelineStageRunner:
                     base = 3 + r * (1 + self._QUEUE_SLOTS)
                     meta[base] = len(q) if r < len(queues) else -1
                     meta[base + 1:base + 1 + len(q)] = torch.tensor(q, dtype=torch.int64)
-                for t in (meta.to(dev), kv["global_end_index"], kv["local_end_index"], kv["k"].to(dev),
-                          kv["v"].to(dev)):
+                names = cache_tensors(kv)
+                for t in (meta.to(dev), kv["global_end_index"], kv["local_end_index"], *(kv[n].to(dev) for n in names)):
                     dist.send(t.contiguous(), dst=dst)
-                kv["k"], kv["v"] = kv["k"][:, :0], kv["v"][:, :0]         # placeholder, as for never-owned blocks
+                kv.update({n: kv[n][:, :0] for n in names})               # placeholder, as for never-owned blocks
                 RingState.invalidate(kv)
             else:
                 rows = pipe.hidden_states.shape[0]
@@ -312,15 +314,16 @@ class PipelineStageRunner:
                 m = meta.tolist()
                 if m[0] != rows:
                     raise RuntimeError("the sender's cache has another number of rows")
-                dtype = pipe.hidden_states.dtype
                 shape = (rows, pipe.kv_cache_length, pipe.num_heads, pipe.head_dim)
+                if "k_exp" in kv:
+                    tensors = ops.q8_cache(rows, pipe.kv_cache_length, pipe.num_heads, dev)
+                else:
+                    tensors = {n: torch.empty(shape, dtype=pipe.hidden_states.dtype, device=dev) for n in ("k", "v")}
                 ge = torch.empty(rows, dtype=torch.int64, device=dev)
                 le = torch.empty(rows, dtype=torch.int64, device=dev)
-                k = torch.empty(shape, dtype=dtype, device=dev)
-                v = torch.empty(shape, dtype=dtype, device=dev)
-                for t in (ge, le, k, v):
+                for t in (ge, le, *(tensors[n] for n in cache_tensors(kv))):
                     dist.recv(t, src=src)
-                kv.update(k=k, v=v, global_end_index=ge, local_end_index=le, current_step=m[1], total_steps=m[2])
+                kv.update(tensors, global_end_index=ge, local_end_index=le, current_step=m[1], total_steps=m[2])
                 RingState.invalidate(kv)              # the host mirror is re-read from the received tensors
                 queues = []
                 for r in range(rows):

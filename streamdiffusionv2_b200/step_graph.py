@@ -87,8 +87,7 @@ def _cache_pointers(layers: Sequence[tuple]) -> List[int]:
     for entry in layers:
         kv = entry[1]
         if kv is not None:            # None: a block of which only the cross-attention half runs here
-            out += [kv["k"].data_ptr(), kv["v"].data_ptr(), kv["global_end_index"].data_ptr(),
-                    kv["local_end_index"].data_ptr()]
+            out += [kv[n].data_ptr() for n in (*CA.cache_tensors(kv), "global_end_index", "local_end_index")]
         if len(entry) > 2 and entry[2] is not None and entry[2].get("is_init"):
             out += [entry[2]["k"].data_ptr(), entry[2]["v"].data_ptr()]
     return out

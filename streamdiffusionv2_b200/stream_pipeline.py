@@ -18,7 +18,8 @@ from typing import Callable, List, Optional, Sequence
 import torch
 import torch.nn as nn
 
-from .causal_attention import HostStarts
+from . import ops
+from .causal_attention import HostStarts, cache_tensors
 
 
 def assign_ints(t: torch.Tensor, values) -> None:
@@ -114,8 +115,12 @@ class StreamPipeline(nn.Module):
     def __init__(self, generator: DiffusionWrapper, text_encoder: Callable, denoising_step_list: Sequence[int],
                  num_transformer_blocks: int, num_heads: int, frame_seq_length: int, num_kv_cache: int,
                  num_sink_tokens: int, adapt_sink_threshold: float = -1, num_frame_per_block: int = 1,
-                 device="cuda", head_dim: int = 128, warp_denoising_step: bool = False, drop_final_zero: bool = True):
+                 device="cuda", head_dim: int = 128, warp_denoising_step: bool = False, drop_final_zero: bool = True,
+                 kv_cache_q8: bool = False):
+        """kv_cache_q8: keep the self-attention K/V in 8 bits (`ops.q8_cache`): half the cache memory, so twice the
+        window or streams per GPU; needs a bf16 model."""
         super().__init__()
+        self.kv_cache_q8 = kv_cache_q8
         self.generator = generator
         self.text_encoder = text_encoder
         self.device = torch.device(device)
@@ -186,9 +191,10 @@ class StreamPipeline(nn.Module):
             blk.self_attn.sink_size = self.num_sink_tokens
             blk.self_attn.adapt_sink_thr = self.adapt_sink_threshold
             shape = [batch_size, self.kv_cache_length, self.num_heads, self.head_dim]
+            tensors = ops.q8_cache(batch_size, self.kv_cache_length, self.num_heads, device) if self.kv_cache_q8 else {
+                n: torch.zeros(shape, dtype=dtype, device=device) for n in ("k", "v")}
             self.kv_cache1.append({
-                "k": torch.zeros(shape, dtype=dtype, device=device),
-                "v": torch.zeros(shape, dtype=dtype, device=device),
+                **tensors,
                 "global_end_index": torch.tensor([0], dtype=torch.long, device=device),
                 "local_end_index": torch.tensor([0], dtype=torch.long, device=device),
                 "total_steps": steps,
@@ -247,18 +253,17 @@ class StreamPipeline(nn.Module):
         for i in range(self.num_transformer_blocks):
             kv, cc = self.kv_cache1[i], self.crossattn_cache[i]
             if torch.distributed.is_available() and torch.distributed.is_initialized():
-                for t in (cc["k"], cc["v"], kv["k"], kv["v"]):
+                for t in (cc["k"], cc["v"], *(kv[n] for n in cache_tensors(kv))):
                     torch.distributed.broadcast(t, src=0)
             if owned_blocks is not None and i not in owned_blocks and unowned == "free":
-                kv["k"], kv["v"] = kv["k"][:, :0], kv["v"][:, :0]
-            kv["k"] = kv["k"].repeat(levels, 1, 1, 1)
-            kv["v"] = kv["v"].repeat(levels, 1, 1, 1)
+                kv.update({n: kv[n][:, :0] for n in cache_tensors(kv)})
+            kv.update({n: kv[n].repeat(levels, *[1] * (kv[n].dim() - 1)) for n in cache_tensors(kv)})
             kv["global_end_index"] = kv["global_end_index"].repeat(levels)
             kv["local_end_index"] = kv["local_end_index"].repeat(levels)
             cc["k"] = cc["k"].expand(levels, -1, -1, -1)
             cc["v"] = cc["v"].expand(levels, -1, -1, -1)
             if owned_blocks is not None and i not in owned_blocks and unowned == "cpu":
-                kv["k"], kv["v"] = kv["k"].cpu(), kv["v"].cpu()
+                kv.update({n: kv[n].cpu() for n in cache_tensors(kv)})
 
         self.hidden_states = torch.zeros((levels, self.num_frame_per_block, *noise.shape[2:]), dtype=noise.dtype,
                                          device=device)

@@ -123,7 +123,7 @@ class DiTBlock(nn.Module):
         self.modulation = nn.Parameter(torch.randn(1, 6, dim) / dim ** 0.5)
 
     def forward(self, x, e, grid_sizes, freqs, context, kv_cache, crossattn_cache, current_start, part="all",
-                modulated=None):
+                modulated=None, block_mask=None, context_lens=None):
         """x [B, L, C]; e [B, F, 6, C] (per-frame modulation from the timestep embedding); `modulated`, when
         given, is `self.modulation.unsqueeze(1) + e` computed by the caller (for all its blocks in one launch).
         `part` runs the block in two halves for pipeline stages that meet inside a block: "attn" ends
@@ -152,8 +152,8 @@ class DiTBlock(nn.Module):
         fuse2 = fused and FUSE_RESIDUAL_LN and x.shape[-1] <= 5120
         xn = None
         if part != "rest":
-            y = self.self_attn(norm_modulate(self.norm1, x, scale_a, shift_a), None, grid_sizes, freqs, None,
-                               kv_cache, current_start, None)
+            y = self.self_attn(norm_modulate(self.norm1, x, scale_a, shift_a), None, grid_sizes, freqs,
+                               block_mask, kv_cache, current_start, None)
             if fuse3 and FUSE_RESIDUAL_LN and part == "all":
                 x, xn = ops.residual_layernorm(x, y, gate_a, frames, self.norm3.eps, weight=self.norm3.weight,
                                                bias=self.norm3.bias)
@@ -164,7 +164,7 @@ class DiTBlock(nn.Module):
         if xn is None:
             xn = ops.layernorm_affine(x, self.norm3.weight, self.norm3.bias, self.norm3.eps) if fuse3 \
                 else self.norm3(x)
-        c = self.cross_attn(xn, context, None, crossattn_cache=crossattn_cache)
+        c = self.cross_attn(xn, context, context_lens, crossattn_cache=crossattn_cache)
         if fuse2:
             x, h = ops.residual_layernorm(x, c, None, frames, self.norm2.eps, scale=scale_f, shift=shift_f)
         else:
@@ -357,6 +357,38 @@ class CausalWanModel(nn.Module):
         if hands_on:
             return x, patched_x_shape
 
+        x = self.head(x, e.unflatten(0, t.shape).unsqueeze(2))
+        return self.unpatchify(x, (frames, gh, gw))
+
+    @torch.no_grad()
+    def forward_clip(self, x, t, context, frames_per_block: Optional[int] = None, context_lens=None,
+                     window_frames: int = -1):
+        """A whole clip in one pass without caches: every block of `frames_per_block` frames (default: the model's
+        num_frame_per_block) attends itself and what came before it (see `causal_attention.block_causal_spans`), as
+        streaming it block by block through a cache that never evicts would.  x [B, C, F, H, W]; t [B, F] timesteps;
+        context [B, Lt, text_dim]; `context_lens`, where given, the prompts' lengths: text tokens past them are not
+        attended.  bf16 on CUDA; inference only.  Returns [B, C, F, H, W]."""
+        device = self.patch_embedding.weight.device
+        if self.freqs.device != device:
+            self.freqs = self.freqs.to(device)
+        x = self.patch_embedding(x)
+        bsz, _, frames, gh, gw = x.shape
+        grid_sizes = torch.tensor([[frames, gh, gw]] * bsz, dtype=torch.long)
+        x = x.flatten(2).transpose(1, 2)
+        e = self.time_embedding(timestep_features(self.freq_dim, t.flatten()).type_as(x))
+        e0 = self.time_projection(e).unflatten(1, (6, self.dim)).unflatten(0, t.shape)
+        if context.shape[1] < self.text_len:
+            pad = context.new_zeros(context.shape[0], self.text_len - context.shape[1], context.shape[2])
+            context = torch.cat([context, pad], dim=1)
+        ctx = self.text_embedding(context)
+        spans = CA.block_causal_spans(frames, gh * gw, frames_per_block or self.num_frame_per_block, device, bsz,
+                                      window_frames)
+        if context_lens is not None:
+            context_lens = torch.as_tensor(context_lens, dtype=torch.int32, device=device)
+        mods = self._stacked_modulation(0, len(self.blocks)) + e0.unsqueeze(0)
+        for i, block in enumerate(self.blocks):
+            x = block(x, e0, grid_sizes, self.freqs, ctx, None, None, 0, modulated=mods[i], block_mask=spans,
+                      context_lens=context_lens)
         x = self.head(x, e.unflatten(0, t.shape).unsqueeze(2))
         return self.unpatchify(x, (frames, gh, gw))
 
