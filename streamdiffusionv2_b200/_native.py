@@ -80,20 +80,19 @@ _SIGNATURES = {
     "sdv2_residual_layernorm": (C.c_int, [C.c_void_p] * 3 + [C.c_int64, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p,
                                                              C.c_int64, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int,
                                                              C.c_float, C.c_void_p]),
-    # views of these four are passed as addresses: building View objects would cost a small call several microseconds
-    "sdv2_rope_kv_append_q8": (C.c_int, [C.c_void_p] * 8 + [C.c_int, C.c_int, C.c_int, C.c_int, C.c_int64,
+    "sdv2_rope_kv_append_q8": (C.c_int, [C.POINTER(View)] * 8 + [C.c_int, C.c_int, C.c_int, C.c_int, C.c_int64,
                                                                   C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int,
                                                                   C.POINTER(C.c_int64), C.POINTER(C.c_int64),
                                                                   C.c_void_p, C.c_void_p, C.c_void_p,
                                                                   C.POINTER(C.c_int64), C.POINTER(C.c_int64),
                                                                   C.c_int, C.c_void_p, C.c_void_p]),
-    "sdv2_kv_read_q8": (C.c_int, [C.c_void_p] * 6 + [C.c_int, C.c_int, C.c_int, C.c_int, C.c_int64,
+    "sdv2_kv_read_q8": (C.c_int, [C.POINTER(View)] * 6 + [C.c_int, C.c_int, C.c_int, C.c_int, C.c_int64,
                                                           C.POINTER(C.c_int64), C.c_int, C.c_void_p]),
-    "sdv2_attn_kvcache_q8": (C.c_int, [C.c_void_p] * 6 + [C.c_int, C.c_int, C.c_int, C.c_int, C.c_int64,
+    "sdv2_attn_kvcache_q8": (C.c_int, [C.POINTER(View)] * 6 + [C.c_int, C.c_int, C.c_int, C.c_int, C.c_int64,
                                                                C.POINTER(C.c_int32), C.c_float, C.c_void_p,
                                                                C.c_size_t, C.c_void_p, C.c_void_p]),
     "sdv2_attn_q8_scratch_bytes": (C.c_size_t, [C.c_int, C.c_int, C.c_int, C.c_int64, C.POINTER(C.c_int32)]),
-    "sdv2_attn_spans": (C.c_int, [C.c_void_p] * 4 + [C.c_int, C.c_int, C.c_int, C.c_int, C.c_int64,
+    "sdv2_attn_spans": (C.c_int, [C.POINTER(View)] * 4 + [C.c_int, C.c_int, C.c_int, C.c_int, C.c_int64,
                                                           C.c_void_p, C.c_int64, C.c_int64, C.c_void_p, C.c_int64,
                                                           C.c_int64, C.c_float, C.c_void_p, C.c_size_t, C.c_void_p,
                                                           C.c_void_p]),
@@ -127,6 +126,27 @@ def lib():
             raise RuntimeError("libsdv2.so ABI version mismatch; rebuild it")
         _lib = l
     return _lib
+
+
+_calls = None
+
+
+def calls():
+    """The PyTorch binding of the 8-bit cache and key-span entry points, bound to the loaded library; raises if it has
+    not been built."""
+    global _calls
+    if _calls is None:
+        l = lib()
+        try:
+            from . import _calls as module
+        except ImportError as e:
+            raise RuntimeError("streamdiffusionv2_b200/_calls.so is missing or does not load: build it with "
+                               "`python -m streamdiffusionv2_b200.build` (there is no fallback path)") from e
+        module.bind(*[C.cast(getattr(l, n), C.c_void_p).value for n in (
+            "sdv2_rope_kv_append_q8", "sdv2_kv_read_q8", "sdv2_attn_q8_scratch_bytes", "sdv2_attn_kvcache_q8",
+            "sdv2_attn_spans_scratch_bytes", "sdv2_attn_spans")], check)
+        _calls = module
+    return _calls
 
 
 def check(code: int, what: str) -> None:

@@ -7,7 +7,6 @@ from __future__ import annotations
 
 import ctypes as C
 import math
-import struct
 from typing import Dict, Optional, Sequence, Tuple
 
 import torch
@@ -301,93 +300,11 @@ def attn_kvcache_simt(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
     return out
 
 
-def _wrong(what: str, name: str, t: torch.Tensor, shape, dtype, device):
-    return ValueError(f"{what}: {name} must be a {dtype} tensor {list(shape)} on {device} with contiguous head_dim, not "
-                      f"{t.dtype} {list(t.shape)} (strides {list(t.stride())}) on {t.device}")
-
-
-def _view4(what: str, name: str, t: torch.Tensor, shape, dtype, device):
-    """(pointer, row, token and head stride) of a [rows, tokens, heads, head_dim] tensor of exactly this shape, type and
-    device.  A size-1 row dimension may carry any stride: it gets a legal one."""
-    st = t.stride()
-    if t.shape != shape or t.dtype is not dtype or t.device != device or st[3] != 1:
-        raise _wrong(what, name, t, shape, dtype, device)
-    return t.data_ptr(), st[0] if shape[0] > 1 else shape[1] * st[1], st[1], st[2]
-
-
-def _view3(what: str, name: str, t: torch.Tensor, shape, device):
-    """The same for the int8 exponents [rows, tokens, heads] of an 8-bit cache."""
-    if t.shape != shape or t.dtype is not torch.int8 or t.device != device:
-        raise _wrong(what, name, t, shape, torch.int8, device)
-    st = t.stride()
-    tok, head = st[1] if shape[1] > 1 else max(1, shape[2]), st[2] if shape[2] > 1 else 1
-    return t.data_ptr(), st[0] if shape[0] > 1 else shape[1] * tok, tok, head
-
-
-def _q8_views(what: str, device, k_cache, v_cache, k_exp, v_exp, rows: int, heads: int, head_dim: int):
-    """Length in tokens and the four views of an 8-bit cache."""
-    if head_dim != 128:
-        raise ValueError(f"{what}: the 8-bit cache has head_dim 128, not {head_dim}")
-    smax = k_cache.shape[1] if k_cache.dim() == 4 else 0
-    s4 = (rows, smax, heads, 128)
-    s3 = s4[:3]
-    u8 = torch.uint8
-    return smax, (*_view4(what, "k_cache", k_cache, s4, u8, device), *_view4(what, "v_cache", v_cache, s4, u8, device),
-                  *_view3(what, "k_exp", k_exp, s3, device), *_view3(what, "v_exp", v_exp, s3, device))
-
-
-_VIEWS = {n: (struct.Struct(f"{4 * n}q").pack, C.c_char * (32 * n)) for n in (4, 6, 8)}
-
-
-def _packed_views(*flat):
-    """Views (four numbers each) back to back in memory: the buffer to keep until the launch and their addresses."""
-    pack, buf = _VIEWS[len(flat) >> 2]
-    arr = buf.from_buffer_copy(pack(*flat))
-    base = C.addressof(arr)
-    return arr, range(base, base + 8 * len(flat), 32)
-
-
-def _launch(name: str, work, device: torch.device, fn, args) -> None:
-    """fn(*args, stream) with `device` current, logged under `name` with `work()` units of work."""
-    idx = device.index
-    if idx is None:
-        raise ValueError(f"{name}: expected CUDA tensors (there is no CPU path)")
-    if idx != torch.cuda.current_device():
-        with torch.cuda.device(idx):
-            return _launch(name, work, device, fn, args)
-    stream = torch._C._cuda_getCurrentRawStream(idx)
-    if _log is None:
-        rc = fn(*args, stream)
-    else:
-        with _Logged(name, work()):
-            rc = fn(*args, stream)
-    if rc != 0:
-        N.check(rc, name)
-
-
-def _call_scratch(nbytes_fn, device: torch.device, *args):
-    """(tensor to keep until the launch, pointer, bytes) of a call's own scratch.  It comes from PyTorch's allocator on
-    the launching stream (a graph's own pool while capturing), so calls on other streams and other recorded graphs never
-    share it."""
-    if device.index is not None and device.index != torch.cuda.current_device():
-        with torch.cuda.device(device.index):
-            return _call_scratch(nbytes_fn, device, *args)
-    nbytes = nbytes_fn(*args)
-    if nbytes == 0:
-        return None, None, 0
-    t = torch.empty(nbytes, dtype=torch.uint8, device=device)
-    return t, t.data_ptr(), nbytes
-
-
-def _status_ptr(device: torch.device):
-    """Address of the device's status word (the first word of `workspace`)."""
-    return workspace(device).data_ptr() if device.index is not None else None
-
-
-def _cuda_device(what: str, t: torch.Tensor) -> torch.device:
-    if t.dim() != 4:
-        raise ValueError(f"{what}: expected a [rows, tokens, heads, head_dim] tensor, not {list(t.shape)}")
-    return t.device
+def _status_ptr(t: torch.Tensor) -> int:
+    """Address of the status word (the first word of `workspace`) of a tensor's device; 0 for host tensors, which the call
+    refuses."""
+    device = t.device
+    return workspace(device).data_ptr() if device.index is not None else 0
 
 
 Q8_MIN_EXP = -126          # smallest exponent of the 8-bit cache format: that of a vector of zeros
@@ -414,43 +331,12 @@ def rope_kv_append_q8(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache
     magnitudes min(rint(|x| / 2^e), 127).  A head vector with a value that is not finite reads back as NaN.
     q, k, v [B, N, H, 128] bf16 or fp32; `index_tensors`, `index_values`, `step_params` as for `rope_kv_append`.
     Returns the roped q, the same bits as `rope_kv_append`'s."""
-    what = "rope_kv_append_q8"
-    dev = _cuda_device(what, q)
-    shape, dtype = q.shape, q.dtype
-    B, n_new, H, D = shape
-    smax, cache = _q8_views(what, dev, k_cache, v_cache, k_exp, v_exp, B, H, D)
-    if q_out is None:
-        q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    if (table.dim() != 3 or table.shape[1:] != (D // 2, 2) or table.dtype is not torch.float64 or table.device != dev
-            or not table.is_contiguous()):
-        raise ValueError(f"{what}: the rope table must be a contiguous float64 [rows, {D // 2}, 2] tensor on {dev}")
-    f, h, w = grid
-    ge_dev = le_dev = ge_val = le_val = params = starts = dsts = None
-    if index_tensors is not None:
-        for t in index_tensors:
-            if t.dtype is not torch.int64 or t.numel() < B or not t.is_contiguous() or t.device != dev:
-                raise ValueError("index tensors must be contiguous int64 with one entry per row, on q's device")
-        ge_dev, le_dev = index_tensors[0].data_ptr(), index_tensors[1].data_ptr()
-    if step_params is not None:
-        if (step_params.dtype is not torch.int64 or not step_params.is_contiguous() or step_params.numel() != 4 * B
-                or step_params.device != dev):
-            raise ValueError("step_params must be a contiguous int64 [4, rows] tensor on the same device")
-        params = step_params.data_ptr()
-    else:
-        if len(start_frames) < B or len(dst_begin) < B:
-            raise ValueError("start_frames and dst_begin need one entry per row")
-        starts, dsts = N.i64_array(start_frames), N.i64_array(dst_begin)
-        if index_tensors is not None:
-            if index_values is None or len(index_values[0]) < B or len(index_values[1]) < B:
-                raise ValueError("index_values need one entry per row")
-            ge_val, le_val = N.i64_array(index_values[0]), N.i64_array(index_values[1])
-    keep, at = _packed_views(*_view4(what, "q", q, shape, dtype, dev), *_view4(what, "k", k, shape, dtype, dev),
-                             *_view4(what, "v", v, shape, dtype, dev), *_view4(what, "q_out", q_out, shape, dtype, dev),
-                             *cache)
-    _launch(what, lambda: B * n_new * H * (4.0 * D * q.element_size() + 2 * (D + 1)), dev, N.lib().sdv2_rope_kv_append_q8,
-            (*at, B, n_new, H, D, smax, table.data_ptr(), table.shape[0], int(f), int(h), int(w), starts, dsts, params, ge_dev,
-             le_dev, ge_val, le_val, N.dtype_code(dtype), _status_ptr(dev)))
-    return q_out
+    args = (q, k, v, k_cache, v_cache, k_exp, v_exp, table, grid, start_frames, dst_begin, q_out, index_tensors, index_values,
+            step_params, _status_ptr(q))
+    if _log is None:
+        return N.calls().append_q8(*args)
+    with _Logged("rope_kv_append_q8", q.numel() * (4.0 * q.element_size() + 2.0 * 129 / 128)):
+        return N.calls().append_q8(*args)
 
 
 def kv_read_q8(k_cache: torch.Tensor, v_cache: torch.Tensor, k_exp: torch.Tensor, v_exp: torch.Tensor,
@@ -458,21 +344,11 @@ def kv_read_q8(k_cache: torch.Tensor, v_cache: torch.Tensor, k_exp: torch.Tensor
                out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """(k, v) [B, tokens, H, 128]: what an 8-bit cache holds of tokens begin[b] .. begin[b] + tokens - 1 of every row,
     in bf16 or fp32 (both exact)."""
-    what = "kv_read_q8"
-    dev = _cuda_device(what, k_cache)
-    B, _, H, D = k_cache.shape
-    smax, cache = _q8_views(what, dev, k_cache, v_cache, k_exp, v_exp, B, H, D)
-    shape = (B, tokens, H, D)
-    if len(begin) < B:
-        raise ValueError("kv_read_q8: begin needs one entry per row")
-    if out is None:
-        out = torch.empty((2,) + shape, dtype=dtype, device=dev).unbind(0)
-    keep, at = _packed_views(*cache, *_view4(what, "out[0]", out[0], shape, dtype, dev),
-                             *_view4(what, "out[1]", out[1], shape, dtype, dev))
-    if B * tokens * H != 0:
-        _launch(what, lambda: B * tokens * H * 2.0 * (D + 1 + D * out[0].element_size()), dev, N.lib().sdv2_kv_read_q8,
-                (*at, B, tokens, H, D, smax, N.i64_array(begin), N.dtype_code(dtype)))
-    return out
+    args = (k_cache, v_cache, k_exp, v_exp, begin, tokens, dtype, out)
+    if _log is None:
+        return N.calls().read_q8(*args)
+    with _Logged("kv_read_q8", 2.0 * k_cache.shape[0] * tokens * k_cache.shape[2] * (129 + 128 * dtype.itemsize)):
+        return N.calls().read_q8(*args)
 
 
 def attn_kvcache_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_exp: torch.Tensor,
@@ -480,27 +356,11 @@ def attn_kvcache_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
                     softmax_scale: Optional[float] = None) -> torch.Tensor:
     """`attn_kvcache` over an 8-bit cache: softmax(q k^T scale) v over the values that cache[b, :seq_lens[b]] holds
     (bf16 q and output).  seq_lens[b] may be 0: that row's output is 0."""
-    what = "attn_kvcache_q8"
-    dev = _cuda_device(what, q)
-    shape = q.shape
-    B, n_q, H, D = shape
-    if q.dtype is not torch.bfloat16:
-        raise ValueError("the tensor-core attention kernel takes bf16")
-    smax, cache = _q8_views(what, dev, k_cache, v_cache, k_exp, v_exp, B, H, D)
-    if out is None:
-        out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    if len(seq_lens) < B:
-        raise ValueError("attn_kvcache_q8: seq_lens needs one entry per row")
-    keep, at = _packed_views(*_view4(what, "q", q, shape, q.dtype, dev), *cache, *_view4(what, "out", out, shape, q.dtype, dev))
-    if q.numel() == 0 or smax == 0:
-        return out.zero_()
-    scale = softmax_scale if softmax_scale is not None else 1.0 / math.sqrt(D)
-    lens = N.i32_array(seq_lens)
-    lib = N.lib()
-    scratch = _call_scratch(lib.sdv2_attn_q8_scratch_bytes, dev, B, n_q, H, smax, lens)
-    _launch(what, lambda: 4.0 * n_q * D * H * float(sum(int(x) for x in seq_lens[:B])), dev, lib.sdv2_attn_kvcache_q8,
-            (*at, B, n_q, H, D, smax, lens, scale, scratch[1], scratch[2], _status_ptr(dev)))
-    return out
+    args = (q, k_cache, v_cache, k_exp, v_exp, seq_lens, out, softmax_scale, _status_ptr(q))
+    if _log is None:
+        return N.calls().attn_q8(*args)
+    with _Logged("attn_kvcache_q8", 4.0 * q.shape[1] * q.shape[2] * q.shape[3] * float(sum(int(x) for x in seq_lens[:q.shape[0]]))):
+        return N.calls().attn_q8(*args)
 
 
 def attn_spans(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, begin: Optional[torch.Tensor], end: torch.Tensor, *,
@@ -510,31 +370,11 @@ def attn_spans(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, begin: Optiona
     stride-0 expands over rows); begin (None: 0) and end int32 [B, N] on the device, any strides (an expanded [B, 1]
     does for one span per row).  Spans are clipped to the keys there are; a query with an empty span gets 0.  K and V of
     keys that no query attends may hold anything."""
-    what = "attn_spans"
-    dev = _cuda_device(what, q)
-    shape, dtype = q.shape, q.dtype
-    B, n_q, H, D = shape
-    if dtype is not torch.bfloat16:
-        raise ValueError("the tensor-core attention kernel takes bf16")
-    S = k.shape[1]
-    kv_shape = (B, S, H, D)
-    if out is None:
-        out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    for name, t in (("end", end), ("begin", begin)):
-        if t is not None and (t.shape != (B, n_q) or t.dtype is not torch.int32 or t.device != dev):
-            raise ValueError(f"attn_spans: {name} must be an int32 tensor {[B, n_q]} on {dev}")
-    keep, at = _packed_views(*_view4(what, "q", q, shape, dtype, dev), *_view4(what, "k", k, kv_shape, dtype, dev),
-                             *_view4(what, "v", v, kv_shape, dtype, dev), *_view4(what, "out", out, shape, dtype, dev))
-    if q.numel() == 0 or S == 0:
-        return out.zero_()
-    scale = softmax_scale if softmax_scale is not None else 1.0 / math.sqrt(D)
-    lib = N.lib()
-    scratch = _call_scratch(lib.sdv2_attn_spans_scratch_bytes, dev, B, n_q, H, S)
-    spans = (None, 0, 0) if begin is None else (begin.data_ptr(), *begin.stride())
-    _launch(what, lambda: 4.0 * B * n_q * D * H * S, dev, lib.sdv2_attn_spans,
-            (*at, B, n_q, H, D, S, *spans, end.data_ptr(), *end.stride(), scale, scratch[1], scratch[2],
-             _status_ptr(dev)))
-    return out
+    args = (q, k, v, begin, end, out, softmax_scale, _status_ptr(q))
+    if _log is None:
+        return N.calls().spans(*args)
+    with _Logged("attn_spans", 4.0 * q.numel() * k.shape[1]):
+        return N.calls().spans(*args)
 
 
 def rmsnorm(x: torch.Tensor, weight: torch.Tensor, eps: float) -> torch.Tensor:
