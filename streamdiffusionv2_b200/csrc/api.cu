@@ -681,8 +681,8 @@ int sdv2_attn_kvcache_q8(const sdv2_view* q, const sdv2_view* k_cache, const sdv
     if (r.slots > 0) r.p.part_meta = r.p.part_o + static_cast<size_t>(r.slots) * sdv2::kFewRows * 128;
     r.p.k_row_mask = k_cache->stride_row > 0 ? -1 : 0;
     r.p.v_row_mask = v_cache->stride_row > 0 ? -1 : 0;
-    if ((rc = make_byte_map(&tm_k, k_cache, rows, cache_tokens, heads, 16)) != SDV2_OK) return rc;
-    if ((rc = make_byte_map(&tm_v, v_cache, rows, cache_tokens, heads, 16)) != SDV2_OK) return rc;
+    if ((rc = make_byte_map(&tm_k, k_cache, rows, cache_tokens, heads, sdv2::kFewStageKeys)) != SDV2_OK) return rc;
+    if ((rc = make_byte_map(&tm_v, v_cache, rows, cache_tokens, heads, sdv2::kFewStageKeys)) != SDV2_OK) return rc;
     e = sdv2::launch_attn_few(tm_k, tm_v, r.p, s);
     return e == cudaSuccess ? SDV2_OK : cuda_fail(e);
   }

@@ -1,7 +1,7 @@
 // Attention of a few queries over the 8-bit cache: up to 16 query rows to a block, bound by reading the cache once.
 //
-// A block's four warps take 16 keys each in turn.  A warp has the bytes of its keys' K and V copied into its own ring of
-// shared-memory stages (TMA, three stages ahead) and works on them with m16n8k16 bf16 products, the 16 query rows as M:
+// A block's four warps take 32 keys each in turn.  A warp has the bytes of its keys' K and V copied into its own ring of
+// shared-memory stages (TMA, the next stage in flight) and works on them with m16n8k16 bf16 products, the 16 query rows as M:
 // the tcgen05 kernel's 128 rows would be empty, and its tiles would have to pass through shared memory as bf16, four
 // times these bytes.  A fragment's order of dims and keys is free as long as both operands agree on it, so a lane loads
 // 16 consecutive bytes of a key and expands them in registers: for K the four dims of a word become one k-step's pair
@@ -31,8 +31,9 @@ using attnx::Item;
 
 constexpr int kRows = kFewRows;       // query rows of a block
 constexpr int kWarps = 4;
-constexpr int kKeys = 16;             // keys of a stage
-constexpr int kStages = 4;
+constexpr int kKeys = kFewStageKeys;  // keys of a stage
+constexpr int kBlocks = kKeys / 8;    // ... in products of eight
+constexpr int kStages = 2;
 constexpr int kStageBytes = kKeys * 128 * 2;
 constexpr int kSmemBar = kWarps * kStages * kStageBytes;
 constexpr int kSmemBytes = kSmemBar + kWarps * kStages * 8 + 16 + 1024;  // barriers, abort flag, alignment
@@ -86,11 +87,10 @@ attn_few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
                                            : static_cast<int>(static_cast<int64_t>(item.part + 1) * n_all / item.parts)) * 128);
   constexpr int kStride = kWarps * kKeys;
   const int first0 = key0 + warp * kKeys;
-  // lanes 0..15 read the K exponent of key lane, lanes 16..31 the V exponent of key lane - 16
-  const sdv2_view& ex = lane < 16 ? p.k_exp : p.v_exp;
-  const int8_t* eb = static_cast<const int8_t*>(ex.ptr) + b * ex.stride_row + h * ex.stride_head;
-  const int64_t e_stride = ex.stride_tok;
-  int exps[kStages];
+  static_assert(kKeys == 32, "a lane has the exponents of one key");
+  const int8_t* keb = static_cast<const int8_t*>(p.k_exp.ptr) + b * p.k_exp.stride_row + h * p.k_exp.stride_head;
+  const int8_t* veb = static_cast<const int8_t*>(p.v_exp.ptr) + b * p.v_exp.stride_row + h * p.v_exp.stride_head;
+  int exp_k[kStages], exp_v[kStages];
   auto load = [&](int stage, int first) {
     if (first >= key1) return;
     if (lane == 0) {
@@ -99,7 +99,9 @@ attn_few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
       tma_load_4d(dst, &tm_k, bar, 0, h, first, b & p.k_row_mask);
       tma_load_4d(dst + kKeys * 128, &tm_v, bar, 0, h, first, b & p.v_row_mask);
     }
-    exps[stage] = eb[static_cast<int64_t>(min(first + (lane & 15), key1 - 1)) * e_stride];
+    const int64_t key = min(first + lane, key1 - 1);
+    exp_k[stage] = keb[key * p.k_exp.stride_tok];
+    exp_v[stage] = veb[key * p.v_exp.stride_tok];
   };
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) load(i, first0 + i * kStride);
@@ -182,50 +184,55 @@ attn_few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
       }
       const uint32_t ks = ring + st * kStageBytes, vs = ks + kKeys * 128;
 
-      // S = Q K^T for two blocks of eight keys; a lane holds keys 2 t4, 2 t4 + 1 of each
-      float s[2][4];
+      // S = Q K^T, eight keys a block; a lane holds keys 2 t4, 2 t4 + 1 of each
+      float s[kBlocks][4];
 #pragma unroll
-      for (int nb = 0; nb < 2; ++nb) s[nb][0] = s[nb][1] = s[nb][2] = s[nb][3] = 0.f;
+      for (int nb = 0; nb < kBlocks; ++nb) s[nb][0] = s[nb][1] = s[nb][2] = s[nb][3] = 0.f;
 #pragma unroll
       for (int hf = 0; hf < 2; ++hf) {
-        const uint4 k0 = ld_shared_v4(ks + chunk_at(g, hf * 4 + t4)), k1 = ld_shared_v4(ks + chunk_at(8 + g, hf * 4 + t4));
+        uint4 kv[kBlocks];
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          uint32_t lo, hi;
-          q8::spread4(word(k0, w), lo, hi);
-          mma(s[0], qa[hf * 4 + w], lo, hi);
-          q8::spread4(word(k1, w), lo, hi);
-          mma(s[1], qa[hf * 4 + w], lo, hi);
+        for (int nb = 0; nb < kBlocks; ++nb) kv[nb] = ld_shared_v4(ks + chunk_at(nb * 8 + g, hf * 4 + t4));
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+#pragma unroll
+          for (int nb = 0; nb < kBlocks; ++nb) {
+            uint32_t lo, hi;
+            q8::spread4(word(kv[nb], w), lo, hi);
+            mma(s[nb], qa[hf * 4 + w], lo, hi);
+          }
+      }
+      // this lane's key: its exponents as factors of a score and of a weight, and R
+      const int left = key1 - first;
+      const int ref_new = max(ref_v, __reduce_max_sync(0xffffffffu, exp_v[st]));
+      float fk = fmaxf(attnx::exp2_int(exp_k[st] + 133 - kQueryExp) * p.scale_log2, 1.17549435e-38f);
+      float fv = attnx::exp2_int(exp_v[st] - ref_new + kWeightExp);
+      if (exp_k[st] == q8::kNotFinite) fk = NAN;
+      if (exp_v[st] == q8::kNotFinite) fv = NAN;
+      if (lane >= left) fv = 0.f;
+#pragma unroll
+      for (int nb = 0; nb < kBlocks; ++nb)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float f = __shfl_sync(0xffffffffu, fk, nb * 8 + 2 * t4 + i);
+          s[nb][i] *= f;
+          s[nb][2 + i] *= f;
         }
-      }
-      // this lane's exponent as a factor, of a score (lanes 0..15) or of a weight, and R
-      const int e = exps[st], left = key1 - first;
-      const int top_v = __reduce_max_sync(0xffffffffu, lane < 16 ? q8::kMinExp : e);
-      const int ref_new = max(ref_v, top_v);
-      float factor = attnx::exp2_int(lane < 16 ? e + 133 - kQueryExp : e - ref_new + kWeightExp);
-      if (lane < 16) factor = fmaxf(factor * p.scale_log2, 1.17549435e-38f);
-      if (e == q8::kNotFinite) factor = NAN;
-      if ((lane & 15) >= left) factor = 0.f;
-      float mx[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int key = (i >> 1) * 8 + 2 * t4 + (i & 1);
-        const float f = __shfl_sync(0xffffffffu, factor, key);
-#pragma unroll
-        for (int r = 0; r < 2; ++r) s[i >> 1][2 * r + (i & 1)] *= f;
-      }
       if (!plain) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) s[i >> 2][i & 3] *= row_fix[(i >> 1) & 1];
+        for (int i = 0; i < 4 * kBlocks; ++i) s[i >> 2][i & 3] *= row_fix[(i >> 1) & 1];
       }
       if (left < kKeys) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 2 * kBlocks; ++i)
           if ((i >> 1) * 8 + 2 * t4 + (i & 1) >= left) s[i >> 1][i & 1] = s[i >> 1][2 + (i & 1)] = -INFINITY;
       }
+      float mx[2];
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        mx[r] = fmaxf(fmaxf(s[0][2 * r], s[0][2 * r + 1]), fmaxf(s[1][2 * r], s[1][2 * r + 1]));
+        mx[r] = fmaxf(s[0][2 * r], s[0][2 * r + 1]);
+#pragma unroll
+        for (int nb = 1; nb < kBlocks; ++nb) mx[r] = fmaxf(mx[r], fmaxf(s[nb][2 * r], s[nb][2 * r + 1]));
         mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
         mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
       }
@@ -245,30 +252,34 @@ attn_few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
           }
         }
       }
-      uint32_t pa[4];
+      uint32_t pa[kBlocks / 2][4];
       const float m_sub[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
 #pragma unroll
-      for (int nb = 0; nb < 2; ++nb) {
-        const float f0 = __shfl_sync(0xffffffffu, factor, 16 + nb * 8 + 2 * t4);
-        const float f1 = __shfl_sync(0xffffffffu, factor, 16 + nb * 8 + 2 * t4 + 1);
+      for (int nb = 0; nb < kBlocks; ++nb) {
+        const float f0 = __shfl_sync(0xffffffffu, fv, nb * 8 + 2 * t4), f1 = __shfl_sync(0xffffffffu, fv, nb * 8 + 2 * t4 + 1);
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
           const float p0 = ex2_approx(s[nb][2 * r] - m_sub[r]), p1 = ex2_approx(s[nb][2 * r + 1] - m_sub[r]);
           l[r] += p0 + p1;
-          pa[nb * 2 + r] = pack_bf16x2(p0 * f0, p1 * f1);
+          pa[nb >> 1][(nb & 1) * 2 + r] = pack_bf16x2(p0 * f0, p1 * f1);
         }
       }
-      // O += P V: this lane's column of every block of eight dims is dim g * 16 + block, its keys are the four above
-      const uint4 v0 = ld_shared_v4(vs + chunk_at(2 * t4, g)), v1 = ld_shared_v4(vs + chunk_at(2 * t4 + 1, g));
-      const uint4 v2 = ld_shared_v4(vs + chunk_at(2 * t4 + 8, g)), v3 = ld_shared_v4(vs + chunk_at(2 * t4 + 9, g));
+      // O += P V, 16 keys a step: this lane's column of every block of eight dims is dim g * 16 + block, its keys are the
+      // four above
 #pragma unroll
-      for (int w = 0; w < 4; ++w)
+      for (int kk = 0; kk < kBlocks / 2; ++kk) {
+        uint4 v[4];
 #pragma unroll
-        for (int d = 0; d < 4; ++d) {
-          const uint32_t sel = 0x4400u + 0x1111u * d;  // byte d of the first key doubled, of the second doubled
-          mma(o[w * 4 + d], pa, __byte_perm(word(v0, w), word(v1, w), sel) & 0x807F807Fu,
-              __byte_perm(word(v2, w), word(v3, w), sel) & 0x807F807Fu);
-        }
+        for (int i = 0; i < 4; ++i) v[i] = ld_shared_v4(vs + chunk_at(kk * 16 + 2 * t4 + (i & 1) + (i >> 1) * 8, g));
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+#pragma unroll
+          for (int d = 0; d < 4; ++d) {
+            const uint32_t sel = 0x4400u + 0x1111u * d;  // byte d of the first key doubled, of the second doubled
+            mma(o[w * 4 + d], pa[kk], __byte_perm(word(v[0], w), word(v[1], w), sel) & 0x807F807Fu,
+                __byte_perm(word(v[2], w), word(v[3], w), sel) & 0x807F807Fu);
+          }
+      }
     }
   }
   __syncthreads();

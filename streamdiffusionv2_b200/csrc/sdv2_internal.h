@@ -218,6 +218,7 @@ int plan_lens(AttnXParams& p, int wave, int min_tiles);
 int plan_spans(AttnXParams& p, int sms);
 constexpr int kFewRows = 16;        // query rows of a block of launch_attn_few; partials: [parts][16][128], [parts][2][16]
 constexpr int kFewBlocksPerSm = 3;
+constexpr int kFewStageKeys = 32;   // tokens of a TMA box
 cudaError_t launch_attn_few(const CUtensorMap& tm_k, const CUtensorMap& tm_v, const AttnXParams& p, cudaStream_t stream);
 cudaError_t launch_attn_q8_expand(const CUtensorMap& tm_q, const AttnXParams& p, cudaStream_t stream);
 cudaError_t launch_attn_lens(const CUtensorMap& tm_q, const CUtensorMap& tm_k, const CUtensorMap& tm_v,
