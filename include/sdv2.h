@@ -328,7 +328,7 @@ int sdv2_residual_layernorm(const void* x, const void* y, const void* gate, int6
  *   (`dtype`; both exact).  begin: host int64[rows], begin[b] + tokens <= cache_tokens.  Cache rows may be broadcast.
  * sdv2_attn_kvcache_q8: sdv2_attn_kvcache over the values the cache holds.  seq_lens[b] may be 0: that row's output is
  *   0.  Cache bytes and exponents at and beyond seq_lens[b] may hold anything.  scratch_dev: at least
- *   sdv2_attn_q8_scratch_bytes() bytes (may be 0: then NULL), 16-byte aligned, no initialisation needed; one call's
+ *   sdv2_attn_q8_scratch_bytes() bytes (may be 0: then NULL), 32-byte aligned, no initialisation needed; one call's
  *   own, calls that may overlap on the GPU need one each.  status_dev as for sdv2_rope_kv_append.
  */
 int sdv2_rope_kv_append_q8(const sdv2_view* q, const sdv2_view* k, const sdv2_view* v, const sdv2_view* q_out,

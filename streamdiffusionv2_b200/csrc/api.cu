@@ -582,6 +582,8 @@ static int fill_q_out(sdv2::AttnXParams& p, const sdv2_view* q, const sdv2_view*
   p.out_stride_row = out->stride_row;
   p.out_stride_tok = out->stride_tok;
   p.out_stride_head = out->stride_head;
+  p.out_wide = ((static_cast<int64_t>(reinterpret_cast<uintptr_t>(out->ptr)) | out->stride_row * 2 | out->stride_tok * 2 |
+                 out->stride_head * 2) & 31) == 0;
   p.scale_log2 = softmax_scale * 1.4426950408889634f;
   p.status = status;
   return SDV2_OK;
@@ -670,7 +672,7 @@ int sdv2_attn_kvcache_q8(const sdv2_view* q, const sdv2_view* k_cache, const sdv
   if ((rc = plan_q8(r, heads)) != SDV2_OK) return rc;
   const size_t need = 2 * r.expanded + (r.few ? few_bytes(r.slots) : partial_bytes(r.slots, r.p.tiles));
   if (need > 0 && (scratch_dev == nullptr || scratch_bytes < need)) return SDV2_ERR_WORKSPACE;
-  if (!aligned16(scratch_dev)) return SDV2_ERR_MISALIGNED;
+  if (reinterpret_cast<uintptr_t>(scratch_dev) & 31u) return SDV2_ERR_MISALIGNED;
   char* scratch = static_cast<char*>(scratch_dev);
   set_partials(r.p, scratch + 2 * r.expanded, r.slots);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -755,7 +757,7 @@ int sdv2_attn_spans(const sdv2_view* q, const sdv2_view* k, const sdv2_view* v, 
   int slots = 0;
   if ((rc = plan_spans(p, &slots)) != SDV2_OK) return rc;
   if (slots > 0 && (scratch_dev == nullptr || scratch_bytes < partial_bytes(slots, p.tiles))) return SDV2_ERR_WORKSPACE;
-  if (!aligned16(scratch_dev)) return SDV2_ERR_MISALIGNED;
+  if (reinterpret_cast<uintptr_t>(scratch_dev) & 31u) return SDV2_ERR_MISALIGNED;
   set_partials(p, scratch_dev, slots);
   p.kv_row_broadcast = k->stride_row == 0 ? 1 : 0;
   p.begin = begin_dev;

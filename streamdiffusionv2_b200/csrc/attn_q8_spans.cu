@@ -679,14 +679,18 @@ attn_x_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
               y[i] = l == 0.f ? 0.f : __uint_as_float(o[i]) * inv;
               if (kQ8) y[i] *= unit;
             }
+            // a thread has a row of its own, so a store of 32 bytes touches half as many sectors as two of 16
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              uint4 v;
-              v.x = pack_bf16x2(y[8 * i + 0], y[8 * i + 1]);
-              v.y = pack_bf16x2(y[8 * i + 2], y[8 * i + 3]);
-              v.z = pack_bf16x2(y[8 * i + 4], y[8 * i + 5]);
-              v.w = pack_bf16x2(y[8 * i + 6], y[8 * i + 7]);
-              *reinterpret_cast<uint4*>(op + c * 32 + i * 8) = v;
+            for (int i = 0; i < 2; ++i) {
+              uint32_t w[8];
+#pragma unroll
+              for (int k = 0; k < 8; ++k) w[k] = pack_bf16x2(y[16 * i + 2 * k], y[16 * i + 2 * k + 1]);
+              if (p.out_wide) {
+                st_global_v8(op + c * 32 + i * 16, w);
+              } else {
+                reinterpret_cast<uint4*>(op + c * 32 + i * 16)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+                reinterpret_cast<uint4*>(op + c * 32 + i * 16)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+              }
             }
           }
         }
@@ -704,9 +708,11 @@ attn_x_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
             tmem_ld32(tO + c * 32, o);
             tmem_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-              *reinterpret_cast<uint4*>(po + c * 32 + i * 4) =
-                  make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t w[8] = {o[8 * i],     o[8 * i + 1], o[8 * i + 2], o[8 * i + 3],
+                                     o[8 * i + 4], o[8 * i + 5], o[8 * i + 6], o[8 * i + 7]};
+              st_global_v8(po + c * 32 + i * 8, w);
+            }
           }
         }
       }

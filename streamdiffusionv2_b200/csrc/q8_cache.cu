@@ -231,9 +231,7 @@ __device__ __forceinline__ void store32(void* p, const uint32_t (&w)[8]) {
     static_cast<uint4*>(p)[1] = make_uint4(w[4], w[5], w[6], w[7]);
     return;
   }
-  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
-               "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
-               : "memory");
+  st_global_v8(p, w);
 }
 
 // A block reads `block_tokens` tokens of one row.  A thread takes 16 bytes of a head vector, of K and of V and of

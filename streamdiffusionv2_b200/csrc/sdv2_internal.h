@@ -192,6 +192,7 @@ struct AttnXParams {
   void* out;
   int64_t out_stride_row, out_stride_tok, out_stride_head;  // elements
   int rows, q_tokens, heads, kv_tokens;
+  int out_wide;          // rows of the output keep 32-byte alignment
   int kv_row_broadcast;  // 1: every row reads K/V row 0
   float scale_log2;      // softmax_scale * log2(e)
   int* status;
