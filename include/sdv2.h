@@ -325,7 +325,8 @@ int sdv2_residual_layernorm(const void* x, const void* y, const void* gate, int6
  *   start_frame / dst_begin (+ index values) with step_params_dev NULL, or step_params_dev (device int64 [4][rows], as
  *   for sdv2_rope_kv_append_indirect) with the host arrays NULL.  head_dim must be 128; dtype is that of q, k, v, q_out.
  * sdv2_kv_read_q8: k_out[b, i], v_out[b, i] = what the cache holds of token begin[b] + i, i < tokens, as bf16 or f32
- *   (`dtype`; both exact).  begin: host int64[rows], begin[b] + tokens <= cache_tokens.  Cache rows may be broadcast.
+ *   (`dtype`; both exact).  begin: host int64[rows], begin[b] + tokens <= cache_tokens.  Cache rows may be broadcast
+ *   (stride_row 0), here and in the attention.  heads <= 8191, there too.
  * sdv2_attn_kvcache_q8: sdv2_attn_kvcache over the values the cache holds.  seq_lens[b] may be 0: that row's output is
  *   0.  Cache bytes and exponents at and beyond seq_lens[b] may hold anything.  scratch_dev: at least
  *   sdv2_attn_q8_scratch_bytes() bytes (may be 0: then NULL), 32-byte aligned, no initialisation needed; one call's

@@ -530,7 +530,7 @@ int sdv2_kv_read_q8(const sdv2_view* k_cache, const sdv2_view* v_cache, const sd
                     int64_t cache_tokens, const int64_t* begin, int dtype, void* stream) {
   if (rows <= 0 || tokens <= 0 || heads <= 0 || cache_tokens <= 0 || begin == nullptr) return SDV2_ERR_INVALID_ARG;
   if (dtype != SDV2_DTYPE_BF16 && dtype != SDV2_DTYPE_F32) return SDV2_ERR_INVALID_ARG;
-  if (head_dim != 128 || rows > SDV2_MAX_ROWS) return SDV2_ERR_UNSUPPORTED_SHAPE;
+  if (head_dim != 128 || rows > SDV2_MAX_ROWS || heads > sdv2::kQ8MaxHeads) return SDV2_ERR_UNSUPPORTED_SHAPE;
   int rc;
   if ((rc = check_view(k_cache, 1, true)) != SDV2_OK || (rc = check_view(v_cache, 1, true)) != SDV2_OK) return rc;
   if ((rc = check_exps(k_exp, true)) != SDV2_OK || (rc = check_exps(v_exp, true)) != SDV2_OK) return rc;
@@ -620,6 +620,7 @@ static int fill_q8(Q8Run& r, int rows, int q_tokens, int heads, int64_t cache_to
   int rc;
   if ((rc = fill_attn_x(r.p, rows, q_tokens, heads, cache_tokens)) != SDV2_OK || (rc = fill_lens(r.p, seq_lens)) != SDV2_OK)
     return rc;
+  if (heads > sdv2::kQ8MaxHeads) return SDV2_ERR_UNSUPPORTED_SHAPE;
   r.few = q_tokens <= kFewQueries;
   if (r.few) r.p.pair_tiles = (q_tokens + sdv2::kFewRows - 1) / sdv2::kFewRows;
   r.group = heads;

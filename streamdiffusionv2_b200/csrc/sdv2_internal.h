@@ -177,6 +177,7 @@ struct Q8AppendParams {
 };
 cudaError_t launch_rope_kv_append_q8(const Q8AppendParams& p, int dtype, cudaStream_t stream);
 
+constexpr int kQ8MaxHeads = 8191;  // of a read: divisions by the 8 x heads lanes of a token are exact up to 2^32
 struct Q8ReadParams {
   sdv2_view k, v, k_exp, v_exp, k_out, v_out;
   int rows, tokens, heads, dtype;

@@ -301,10 +301,12 @@ def attn_kvcache_simt(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
 
 
 def _status_ptr(t: torch.Tensor) -> int:
-    """Address of the status word (the first word of `workspace`) of a tensor's device; 0 for host tensors, which the call
-    refuses."""
-    device = t.device
-    return workspace(device).data_ptr() if device.index is not None else 0
+    """Address of the status word (the first word of `workspace`) of a tensor's device; 0 (not reported) for host tensors,
+    which the call refuses, and while a graph is recorded before there is a workspace, which must not come from its pool."""
+    idx = t.device.index
+    if idx is None or (idx not in _workspaces and torch.cuda.is_current_stream_capturing()):
+        return 0
+    return workspace(t.device).data_ptr()
 
 
 Q8_MIN_EXP = -126          # smallest exponent of the 8-bit cache format: that of a vector of zeros
@@ -355,7 +357,9 @@ def attn_kvcache_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
                     v_exp: torch.Tensor, seq_lens: Sequence[int], *, out: Optional[torch.Tensor] = None,
                     softmax_scale: Optional[float] = None) -> torch.Tensor:
     """`attn_kvcache` over an 8-bit cache: softmax(q k^T scale) v over the values that cache[b, :seq_lens[b]] holds
-    (bf16 q and output).  seq_lens[b] may be 0: that row's output is 0."""
+    (bf16 q and output).  seq_lens[b] may be 0: that row's output is 0.  Cache rows may be broadcast.  Scratch comes from
+    PyTorch's allocator; above 768 queries it holds bf16 K and V of a group of heads, about 1 GiB at most (one head at
+    least).  No gradient is recorded."""
     args = (q, k_cache, v_cache, k_exp, v_exp, seq_lens, out, softmax_scale, _status_ptr(q))
     if _log is None:
         return N.calls().attn_q8(*args)
@@ -369,7 +373,7 @@ def attn_spans(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, begin: Optiona
     block-causal clips, clips packed into one row, windows.  q [B, N, H, 128], k / v [B, S, H, 128] bf16 (k / v may be
     stride-0 expands over rows); begin (None: 0) and end int32 [B, N] on the device, any strides (an expanded [B, 1]
     does for one span per row).  Spans are clipped to the keys there are; a query with an empty span gets 0.  K and V of
-    keys that no query attends may hold anything."""
+    keys that no query attends may hold anything.  No gradient is recorded."""
     args = (q, k, v, begin, end, out, softmax_scale, _status_ptr(q))
     if _log is None:
         return N.calls().spans(*args)

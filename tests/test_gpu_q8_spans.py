@@ -310,6 +310,49 @@ def test_q8_attention_strided_views_scale_and_growing_logits():
     assert not bool(buf[:, 0].any()) and not bool(buf[:, :, 1::2].any())
 
 
+@pytest.mark.parametrize("queries", [1, 100, 900])
+def test_q8_attention_cache_rows_broadcast_and_heads_outermost(queries):
+    """The three ways the attention runs (few queries, expanded in the kernel, expanded first) over one cache row shared by
+    all rows, and over caches whose heads lie outside the tokens."""
+    ops = _ops()
+    S, H = 333, 3
+    c = _held_cache(1, S, H, 41, spread=1.0)
+    q = _randn(9, 2, queries, H, 128).to(torch.bfloat16)
+    lens = [333, 150]
+    wide = {n: t.to(DEV).expand(2, *t.shape[1:]) for n, t in c.items()}
+    out = ops.attn_kvcache_q8(q.to(DEV), wide["k"], wide["v"], wide["k_exp"], wide["v_exp"], lens)
+    full = {n: t.expand(2, *t.shape[1:]) for n, t in c.items()}
+    _check_q8(full, q, lens, out)
+    outer = {n: t.transpose(1, 2).contiguous().to(DEV).transpose(1, 2) for n, t in full.items()}
+    out = ops.attn_kvcache_q8(q.to(DEV).transpose(1, 2).contiguous().transpose(1, 2), outer["k"], outer["v"], outer["k_exp"],
+                              outer["v_exp"], lens)
+    _check_q8(full, q, lens, out)
+
+
+@pytest.mark.parametrize("queries", [2, 40, 800])
+def test_8_bit_cache_with_offsets_past_32_bits(queries):
+    """Tokens 5 MB apart: 1100 of them reach past 2^32 bytes.  Written, read back and attended there."""
+    ops = _ops()
+    S, H, n, step = 1100, 2, 6, 5 << 20
+    big = torch.zeros(S * step, dtype=torch.uint8, device=DEV)
+    view = lambda off: big[off:].as_strided((1, S, H, 128), (S * step, step, 128, 1))  # noqa: E731
+    c = _held_cache(1, S, H, 51)
+    d = {"k": view(0), "v": view(1 << 20)}
+    for name in ("k", "v"):
+        d[name].copy_(c[name])
+        d[name + "_exp"] = big[(2 if name == "k" else 3) << 20:].view(torch.int8).as_strided((1, S, H), (S * step, step, 1))
+        d[name + "_exp"].copy_(c[name + "_exp"])
+    k, v = (_randn(s, 1, n, H, 128).to(torch.bfloat16) for s in (1, 2))
+    want = _expected(c, k, v, (1, 2, 3), [5], [S - n])
+    _append(d, k.to(DEV), k.to(DEV), v.to(DEV), (1, 2, 3), [5], [S - n])
+    _same_cache(d, want)
+    kr, _ = ops.kv_read_q8(d["k"], d["v"], d["k_exp"], d["v_exp"], [S - 2 * n], 2 * n)
+    assert torch.equal(kr.double().cpu(), ref.values(want["k"][:, S - 2 * n:], want["k_exp"][:, S - 2 * n:]))
+    q = _randn(3, 1, queries, H, 128).to(torch.bfloat16)
+    _check_q8(want, q, [S], ops.attn_kvcache_q8(q.to(DEV), d["k"], d["v"], d["k_exp"], d["v_exp"], [S]))
+    del big, d
+
+
 # ------------------------------------------------------------------------------------------------ attention, spans
 def _spans(kind, rows, n, S, seed=0):
     g = torch.Generator().manual_seed(seed)
@@ -394,6 +437,22 @@ def test_spans_attention_strides_broadcast_and_scale():
     wide = ops.attn_spans(qd, kd, vd, None, lens.to(DEV).expand(B, n))
     _check_spans(q, k, v, torch.zeros(B, n), lens.expand(B, n), wide)
     assert not bool(wide[1].any())
+
+
+@pytest.mark.parametrize("n,S", [(200, 500), (300, 1700)])
+def test_spans_attention_heads_outermost_and_offsets_past_32_bits(n, S):
+    ops = _ops()
+    H, step = 2, 2 << 20                                    # elements between tokens: 4 MB
+    q, k, v = (_randn(s, 1, m, H, 128).to(torch.bfloat16) for s, m in ((1, n), (2, S), (3, S)))
+    begin, end = _spans("free", 1, n, S, seed=3)
+    outer = [t.transpose(1, 2).contiguous().to(DEV).transpose(1, 2) for t in (q, k, v)]
+    _check_spans(q, k, v, begin, end, ops.attn_spans(*outer, begin.to(DEV), end.to(DEV)))
+    big = torch.zeros(S * step, dtype=torch.bfloat16, device=DEV)
+    kd, vd = (big[off:].as_strided((1, S, H, 128), (S * step, step, 128, 1)) for off in (0, 1 << 20))
+    kd.copy_(k)
+    vd.copy_(v)
+    _check_spans(q, k, v, begin, end, ops.attn_spans(q.to(DEV), kd, vd, begin.to(DEV), end.to(DEV)))
+    del big, kd, vd
 
 
 def test_span_attention_over_whole_rows_agrees_with_the_cache_kernel():

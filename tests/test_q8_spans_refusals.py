@@ -46,12 +46,12 @@ def test_read_refusals(native):
     N = native
     lib = N.lib()
 
-    def call(rows=1, tokens=2, hd=128, cache=8, begin=(0,), dtype=0, out=None):
-        return lib.sdv2_kv_read_q8(*[_view(N)] * 4, out or _view(N), _view(N), rows, tokens, 1, hd, cache,
+    def call(rows=1, tokens=2, hd=128, cache=8, begin=(0,), dtype=0, out=None, heads=1):
+        return lib.sdv2_kv_read_q8(*[_view(N)] * 4, out or _view(N), _view(N), rows, tokens, heads, hd, cache,
                                    N.i64_array(begin) if begin is not None else None, dtype, None)
     assert call(tokens=0) == -1 and call(rows=0) == -1 and call(begin=None) == -1
     assert call(begin=[7]) == -1 and call(begin=[-1]) == -1 and call(tokens=9) == -1
-    assert call(hd=64) == -2 and call(rows=65, begin=[0] * 65) == -2
+    assert call(hd=64) == -2 and call(rows=65, begin=[0] * 65) == -2 and call(heads=8192) == -2
     assert call(dtype=3) == -1 and call(out=_view(N, ptr=0x1002)) == -3 and call(out=_view(N, tok=129)) == -3
 
 
@@ -73,7 +73,7 @@ def test_attention_refusals(native):
         assert call(scale=0.0) == -1 and call(scale=float("nan")) == -1 and call(scale=float("inf")) == -1
         assert call(k=_view(N, ptr=0x1008)) == -3
     assert q8(lens=None) == -1 and q8(lens=[9]) == -1 and q8(lens=[-1]) == -1 and q8(cache=0) == -1
-    assert q8(rows=65, lens=[1] * 65) == -2 and q8(q=_view(N, row=0)) == -1
+    assert q8(rows=65, lens=[1] * 65) == -2 and q8(heads=8192) == -2 and q8(q=_view(N, row=0)) == -1
     assert spans(end=None) == -1 and spans(end=0x5002) == -1 and spans(begin=0x5001) == -1
     assert spans(strides=(-1, 0)) == -1 and spans(strides=(0, -1)) == -1 and spans(keys=0) == -1
     assert spans(k=_view(N, row=0)) == -1                    # K broadcast over rows but V not
