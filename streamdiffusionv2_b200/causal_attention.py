@@ -122,7 +122,8 @@ class KeySpans(NamedTuple):
 def block_causal_spans(frames: int, frame_tokens: int, frames_per_block: int, device, rows: int = 1,
                        window_frames: int = -1) -> KeySpans:
     """Spans of a clip processed in one pass: a token attends its own block of frames and every block before it
-    (the training branch's mask, models/wan/causal_model.py:220-249), with window_frames > 0 only from window_frames frames before its block's end."""
+    (the training branch's mask, models/wan/causal_model.py:220-249), with window_frames > 0 only the last window_frames
+    frames up to its block's end."""
     t = torch.arange(frames * frame_tokens, device=device)
     block = frames_per_block * frame_tokens
     end = ((t // block + 1) * block).clamp_max(frames * frame_tokens)
@@ -151,6 +152,9 @@ def cached_attention(attn_module, q, k, v, grid_sizes, freqs, kv_cache, current_
     (weight_q, weight_k, eps) q and k are the raw projections and their RMS norm
     (causal_model.py:212-214) runs inside the append launch."""
     B, n_new, H, D = q.shape
+    q8 = "k_exp" in kv_cache
+    if q8 and q.dtype != torch.bfloat16:     # before the cache is written
+        raise ValueError(f"attention over an 8-bit cache takes bf16 tensors, not {q.dtype}")
     f, gh, gw = (int(x) for x in grid_sizes[0].tolist())
     frame_tokens = gh * gw
     starts = host_starts(current_start, B)
@@ -163,7 +167,6 @@ def cached_attention(attn_module, q, k, v, grid_sizes, freqs, kv_cache, current_
     index_tensors = (kv_cache["global_end_index"], kv_cache["local_end_index"])
     sink_tokens = attn_module.sink_size * frame_tokens
     adaptive = sink_tokens > 0 and attn_module.adapt_sink_thr > -1 and n_new <= frame_tokens
-    q8 = "k_exp" in kv_cache
     if q8 and norm is not None:          # the 8-bit append takes normalised q and k
         q, k = (ops.rmsnorm(t.flatten(2), w, norm[2]).view(B, n_new, H, D) for t, w in ((q, norm[0]), (k, norm[1])))
         norm = None

@@ -551,7 +551,7 @@ int sdv2_kv_read_q8(const sdv2_view* k_cache, const sdv2_view* v_cache, const sd
 
 static int fill_attn_x(sdv2::AttnXParams& p, int rows, int q_tokens, int heads, int64_t kv_tokens) {
   if (rows <= 0 || q_tokens <= 0 || heads <= 0 || kv_tokens <= 0) return SDV2_ERR_INVALID_ARG;
-  if (rows > SDV2_MAX_ROWS || heads > 65535 || kv_tokens > 0x7FFFFF00LL || q_tokens > 0x7FFFFF00) return SDV2_ERR_UNSUPPORTED_SHAPE;
+  if (rows > SDV2_MAX_ROWS || heads > 65535 || kv_tokens > 0x7FFFF000LL || q_tokens > 0x7FFFF000) return SDV2_ERR_UNSUPPORTED_SHAPE;
   memset(&p, 0, sizeof(p));
   p.rows = rows;
   p.q_tokens = q_tokens;
@@ -577,14 +577,14 @@ static int fill_q_out(sdv2::AttnXParams& p, const sdv2_view* q, const sdv2_view*
   if (head_dim != 128) return SDV2_ERR_UNSUPPORTED_SHAPE;
   int rc;
   if ((rc = check_view(q, 2, false)) != SDV2_OK || (rc = check_view(out, 2, false)) != SDV2_OK) return rc;
-  if (!(softmax_scale > 0.f) || !isfinite(softmax_scale)) return SDV2_ERR_INVALID_ARG;
+  p.scale_log2 = softmax_scale * 1.4426950408889634f;
+  if (!(softmax_scale > 0.f) || !isfinite(p.scale_log2)) return SDV2_ERR_INVALID_ARG;
   p.out = out->ptr;
   p.out_stride_row = out->stride_row;
   p.out_stride_tok = out->stride_tok;
   p.out_stride_head = out->stride_head;
   p.out_wide = ((static_cast<int64_t>(reinterpret_cast<uintptr_t>(out->ptr)) | out->stride_row * 2 | out->stride_tok * 2 |
                  out->stride_head * 2) & 31) == 0;
-  p.scale_log2 = softmax_scale * 1.4426950408889634f;
   p.status = status;
   return SDV2_OK;
 }

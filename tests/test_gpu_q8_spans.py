@@ -248,6 +248,45 @@ def test_q8_attention_ignores_what_lies_behind_the_length():
     _check_q8(c, q, lens, out)
 
 
+@pytest.mark.parametrize("queries", [1, 32, 33, 900])
+def test_q8_attention_ignores_junk_behind_the_length_and_in_scratch(queries):
+    """As above for few queries and for many, whose bf16 scratch takes over memory that was full of NaN."""
+    ops = _ops()
+    lens = [1, 0, 500, 333]
+    c = _held_cache(4, 512, 2, 4)
+    junk = _garbage_cache(4, 512, 2)
+    for b, n in enumerate(lens):
+        for name in c:
+            c[name][b, n:] = junk[name][b, n:]
+        c["v_exp"][b, n:] = -128
+        c["k_exp"][b, n:] = -128
+    q = _randn(5, 4, queries, 2, 128).to(torch.bfloat16)
+    d, qd = _cuda(c), q.to(DEV)
+    dirt = [torch.full((n >> 2,), float("nan"), device=DEV) for n in (4 << 20, 2 << 20, 1 << 20, 512 << 10) for _ in range(4)]
+    del dirt
+    out = ops.attn_kvcache_q8(qd, d["k"], d["v"], d["k_exp"], d["v_exp"], lens)
+    assert bool(torch.isfinite(out).all()) and not out[1].any()
+    _check_q8(c, q, lens, out)
+
+
+def test_q8_attention_in_groups_of_heads():
+    """Many queries over a cache too large to expand at once: 23 heads in groups of 12 and 11, one row nearly empty."""
+    ops = _ops()
+    S, H, n, lens = 50000, 23, 800, [50000, 3]
+    g = torch.Generator(DEV).manual_seed(7)
+    d = {x: torch.randint(0, 256, (2, S, H, 128), generator=g, dtype=torch.uint8, device=DEV) for x in ("k", "v")}
+    d.update({x + "_exp": torch.randint(-8, -5, (2, S, H), generator=g, dtype=torch.int8, device=DEV) for x in ("k", "v")})
+    q = torch.randn(2, n, H, 128, generator=g, device=DEV).to(torch.bfloat16)
+    out = ops.attn_kvcache_q8(q, d["k"], d["v"], d["k_exp"], d["v_exp"], lens)
+    some = [0, 11, 12, 22]
+    for b, end in enumerate(lens):
+        for h in some:                                     # the reference in 64 bits, a head at a time
+            k, v = (ref.values(d[x][b:b + 1, :end, h:h + 1], d[x + "_exp"][b:b + 1, :end, h:h + 1]) for x in ("k", "v"))
+            hi = torch.full((1, n), end)
+            want, weight = ref.span_attention(q[b:b + 1, :, h:h + 1], k, v, torch.zeros_like(hi), hi, None)
+            ref.check_attention(out[b:b + 1, :, h:h + 1], want, weight, end, [end])
+
+
 @pytest.mark.parametrize("queries", [1, 200])
 def test_q8_attention_exponents_far_apart(queries):
     """V scales that grow and shrink along the cache by 2^100 (the accumulator changes its unit), a V that is 0 for

@@ -71,6 +71,7 @@ def test_attention_refusals(native):
         assert call(hd=64) == -2
         assert call(heads=65536) == -2 and call(n=2 ** 31 - 1) == -2
         assert call(scale=0.0) == -1 and call(scale=float("nan")) == -1 and call(scale=float("inf")) == -1
+        assert call(scale=3e38) == -1                        # infinite in log2 units
         assert call(k=_view(N, ptr=0x1008)) == -3
     assert q8(lens=None) == -1 and q8(lens=[9]) == -1 and q8(lens=[-1]) == -1 and q8(cache=0) == -1
     assert q8(rows=65, lens=[1] * 65) == -2 and q8(heads=8192) == -2 and q8(q=_view(N, row=0)) == -1
@@ -112,3 +113,12 @@ def test_wrappers_refuse_wrong_tensors(native):
                  (q, q, q, end[:, :3], end), (q, q, q, None, end[:1])):
         with pytest.raises(ValueError):
             ops.attn_spans(*args)
+
+
+def test_an_8_bit_cache_refuses_fp32_models_before_it_is_written(native):
+    from streamdiffusionv2_b200 import causal_attention as CA, ops
+    cache = dict(ops.q8_cache(1, 8, 2, "cpu"), global_end_index=torch.zeros(1, dtype=torch.int64),
+                 local_end_index=torch.zeros(1, dtype=torch.int64))
+    q = torch.zeros(1, 4, 2, 128)
+    with pytest.raises(ValueError, match="bf16"):
+        CA.cached_attention(None, q, q, q, torch.tensor([[1, 2, 2]]), None, cache, 0)
