@@ -567,7 +567,7 @@ static int fill_lens(sdv2::AttnXParams& p, const int32_t* seq_lens) {
   if (seq_lens == nullptr) return SDV2_ERR_INVALID_ARG;
   for (int b = 0; b < p.rows; ++b) {
     if (seq_lens[b] < 0 || seq_lens[b] > p.kv_tokens) return SDV2_ERR_INVALID_ARG;
-    p.seq_lens[b] = seq_lens[b];
+    p.by_length[b] = {b, seq_lens[b], 0, 0, 0};
   }
   return SDV2_OK;
 }
@@ -622,7 +622,8 @@ static int fill_q8(Q8Run& r, int rows, int q_tokens, int heads, int64_t cache_to
     return rc;
   if (heads > sdv2::kQ8MaxHeads) return SDV2_ERR_UNSUPPORTED_SHAPE;
   r.few = q_tokens <= kFewQueries;
-  if (r.few) r.p.pair_tiles = (q_tokens + sdv2::kFewRows - 1) / sdv2::kFewRows;
+  r.p.few_rows = q_tokens <= 8 ? 8 : sdv2::kFewRows;
+  if (r.few) r.p.pair_tiles = (q_tokens + r.p.few_rows - 1) / r.p.few_rows;
   r.group = heads;
   r.longest = 0;
   r.expanded = 0;

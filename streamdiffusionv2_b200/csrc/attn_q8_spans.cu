@@ -193,6 +193,7 @@ __device__ __forceinline__ Item find_item(const AttnXParams& p, int i) {
   it.tile = p.pair_tiles - 1 - tile / per;
   it.h = tile % per % p.heads;
   it.b = tile % per / p.heads;
+  it.len = 0;
   return it;
 }
 
@@ -294,7 +295,7 @@ attn_x_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
   }
   const uint32_t tmem = static_cast<uint32_t>(words[kWordTmem]);
   // the keys that some row attends, the key tiles they lie in, and this item's share of those
-  const int key_lo = kSpans ? words[kWordLo] : 0, key_hi = kSpans ? words[kWordHi] : p.seq_lens[b];
+  const int key_lo = kSpans ? words[kWordLo] : 0, key_hi = kSpans ? words[kWordHi] : item.len;
   const int tile_lo = kSpans && key_lo < key_hi ? key_lo / kBN : 0;
   const int n_kv_all = key_lo < key_hi ? (key_hi + kBN - 1) / kBN - tile_lo : 0;
   const int j0 = tile_lo + (item.part < 0 ? 0 : static_cast<int>(static_cast<int64_t>(item.part) * n_kv_all / item.parts));

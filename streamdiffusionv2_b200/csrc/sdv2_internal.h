@@ -202,13 +202,16 @@ struct AttnXParams {
   int tiles;             // 128-row query tiles that a CTA has (spans: 1 or 2, else 2)
   int pair_tiles, n_tiles;  // CTAs' worth of query rows per (head, row); of them in all
   int n_full, n_parts;   // tiles [0, n_full) run whole, the others in parts, n_parts of them in all
+  int few_rows;          // launch_attn_few: query rows of a block, 8 or 16
   int split;             // spans: parts of each of the others; lengths: the most parts of one of them
   // 8-bit cache, lengths: rows longest first, parts[r] parts for the tiles of a row
   sdv2_view q, k, v, k_exp, v_exp;
   int k_row_mask, v_row_mask;      // 0: every row reads row 0 of K / V, else all ones
-  int seq_lens[SDV2_MAX_ROWS];     // by row
-  int order[SDV2_MAX_ROWS];        // rows, longest first; the arrays below go by place in this order
-  int tail_tile0[SDV2_MAX_ROWS], item0[SDV2_MAX_ROWS], parts[SDV2_MAX_ROWS];
+  // longest row first; what a CTA needs of its row lies together (a line of the parameter bank costs some 400 cycles)
+  struct Row {
+    int row, len;
+    int tail_tile0, item0, parts;  // first of its tail tiles, first of their items, items of each
+  } by_length[SDV2_MAX_ROWS];
   // spans
   const int* begin;  // null: 0
   const int* end;
@@ -218,7 +221,7 @@ constexpr size_t kAttnXPartFloats = 128 * 128 + 3 * 128;  // of one query tile
 // Fill in how the work is cut up; returns the partial-result slots needed (0: none) or -1 (too many tiles).
 int plan_lens(AttnXParams& p, int wave, int min_tiles);
 int plan_spans(AttnXParams& p, int sms);
-constexpr int kFewRows = 16;        // query rows of a block of launch_attn_few; partials: [parts][16][128], [parts][2][16]
+constexpr int kFewRows = 16;        // most query rows of a block of launch_attn_few; partials: [parts][16][128], [parts][2][16]
 constexpr int kFewBlocksPerSm = 3;
 constexpr int kFewStageKeys = 32;   // tokens of a TMA box
 cudaError_t launch_attn_few(const CUtensorMap& tm_k, const CUtensorMap& tm_v, const AttnXParams& p, cudaStream_t stream);
