@@ -261,6 +261,7 @@ attn_x_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
     tmem_alloc(smem_u32(const_cast<int*>(words + kWordTmem)), Sh::kTmemCols);
     tmem_relinquish();
   }
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the merging kernel may be set up meanwhile
   // this thread's query row (softmax warps) and its span, clipped to the keys there are; for the threads of query tile 0
   // that of the row 128 further on too
   constexpr int kSoftmaxWarp0 = Sh::kSoftmaxWarp0;
@@ -740,6 +741,7 @@ __global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ At
   const Item item =
       find_item<kSpans>(p, kSpans ? p.n_full + static_cast<int>(blockIdx.x) * p.split : first_item_lens(p, blockIdx.x));
   const int q_row = item.tile * (kTiles * kBM) + stage * kBM + row;
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // the parts are complete
   if (item.part < 0 || q_row >= p.q_tokens) return;
   const float* pm = p.part_meta + (static_cast<size_t>(item.slot) * kTiles + stage) * (3 * kBM) + row;
   const float* po = p.part_o + (static_cast<size_t>(item.slot) * kTiles + stage) * (kBM * kHD) + row * kHD + c0;
@@ -795,8 +797,8 @@ cudaError_t launch(const CUtensorMap& tm_q, const CUtensorMap& tm_k, const CUten
   e = cudaGetLastError();
   if (e != cudaSuccess || p.split == 1) return e;
   const int merged = p.n_tiles - p.n_full;
-  combine_kernel<kMode, kTiles><<<dim3(merged, kTiles == 2 && p.q_tokens > kBM ? 2 : 1, kBM / 32), 256, 0, stream>>>(p);
-  return cudaGetLastError();
+  return launch_dependent(combine_kernel<kMode, kTiles>, dim3(merged, kTiles == 2 && p.q_tokens > kBM ? 2 : 1, kBM / 32), dim3(256),
+                          stream, p);
 }
 
 }  // namespace attnx
