@@ -471,7 +471,7 @@ cudaError_t launch(const CUtensorMap& tm_k, const CUtensorMap& tm_v, const AttnX
   attn_few_kernel<kN><<<p.n_full + p.n_parts, kWarps * 32, kSmemBytes, stream>>>(tm_k, tm_v, p);
   e = cudaGetLastError();
   if (e != cudaSuccess || p.split == 1) return e;
-  return launch_dependent(combine_few_kernel, dim3(p.n_tiles - p.n_full, min(p.q_tokens, p.few_rows)), dim3(256), stream, p);
+  return launch_chained(combine_few_kernel, dim3(p.n_tiles - p.n_full, min(p.q_tokens, p.few_rows)), dim3(256), 0, stream, true, p);
 }
 
 }  // namespace few

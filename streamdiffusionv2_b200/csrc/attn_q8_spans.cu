@@ -450,6 +450,7 @@ attn_x_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
         tma_load_4d(base + slot_off(it), tm, full_bar, 0, h, (j0 + kv_tile) * kBN, bk);
         tma_load_4d(base + slot_off(it) + kHalfTile, tm, full_bar, 64, h, (j0 + kv_tile) * kBN, bk);
       };
+      if (kMode == kModeLens) asm volatile("griddepcontrol.wait;" ::: "memory");  // the keys and values are expanded
       mbar_expect_tx(bar(kBarK0Full), kTileBytes);
       load_tile(&tm_k, 0, 0, bar(kBarK0Full));
       bool ok = true;
@@ -792,13 +793,13 @@ cudaError_t launch(const CUtensorMap& tm_q, const CUtensorMap& tm_k, const CUten
   if (e == cudaSuccess) e = smem_grant.ensure(attn_x_kernel<kMode, kTiles>, static_cast<int>(Shape<kMode, kTiles>::kSmemBytes), di.device);
   if (e != cudaSuccess) return e;
   const int items = p.n_full + p.n_parts;
-  attn_x_kernel<kMode, kTiles><<<items, Shape<kMode, kTiles>::kThreads, Shape<kMode, kTiles>::kSmemBytes, stream>>>(
-      tm_q, tm_k, tm_v, p);
-  e = cudaGetLastError();
+  // kModeLens follows kv_read_q8_kernel, behind whose last blocks its set-up passes
+  e = launch_chained(attn_x_kernel<kMode, kTiles>, dim3(items), dim3(Shape<kMode, kTiles>::kThreads),
+                     Shape<kMode, kTiles>::kSmemBytes, stream, kMode == kModeLens, tm_q, tm_k, tm_v, p);
   if (e != cudaSuccess || p.split == 1) return e;
   const int merged = p.n_tiles - p.n_full;
-  return launch_dependent(combine_kernel<kMode, kTiles>, dim3(merged, kTiles == 2 && p.q_tokens > kBM ? 2 : 1, kBM / 32), dim3(256),
-                          stream, p);
+  return launch_chained(combine_kernel<kMode, kTiles>, dim3(merged, kTiles == 2 && p.q_tokens > kBM ? 2 : 1, kBM / 32), dim3(256),
+                        0, stream, true, p);
 }
 
 }  // namespace attnx

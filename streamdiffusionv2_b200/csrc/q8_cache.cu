@@ -238,6 +238,7 @@ __device__ __forceinline__ void store32(void* p, const uint32_t (&w)[8]) {
 // kReadUnroll vectors at a time, and writes them as whole 32-byte sectors.
 template <bool kBf16, bool kWide>
 __global__ void __launch_bounds__(256) kv_read_q8_kernel(const __grid_constant__ Q8ReadParams p) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // an attention that follows may be set up meanwhile
   const int b = blockIdx.y;
   const int t0 = blockIdx.x * p.block_tokens;
   const int n = min(p.block_tokens, p.count[b] - t0) * p.row_vecs;

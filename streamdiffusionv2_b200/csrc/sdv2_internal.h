@@ -147,19 +147,21 @@ __device__ __forceinline__ uint32_t rms_scale_pair(uint32_t x, float rstd, uint3
 }
 #endif
 
-// Launch `kernel` so that its set-up overlaps the end of the kernel before it on the stream; it has to wait for that
-// kernel's results with griddepcontrol.wait.
+// Launch `kernel`; with `early` so that its set-up overlaps the end of the kernel before it on the stream, for whose
+// results it then has to wait with griddepcontrol.wait.
 template <typename... Params, typename... Args>
-cudaError_t launch_dependent(void (*kernel)(Params...), dim3 grid, dim3 block, cudaStream_t stream, const Args&... args) {
+cudaError_t launch_chained(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem_bytes, cudaStream_t stream, bool early,
+                           const Args&... args) {
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t config = {};
   config.gridDim = grid;
   config.blockDim = block;
+  config.dynamicSmemBytes = smem_bytes;
   config.stream = stream;
   config.attrs = &attr;
-  config.numAttrs = 1;
+  config.numAttrs = early ? 1 : 0;
   return cudaLaunchKernelEx(&config, kernel, args...);
 }
 
