@@ -821,8 +821,13 @@ cudaError_t launch_attn_spans(const CUtensorMap& tm_q, const CUtensorMap& tm_k, 
 
 // Spans live on the device, so the host cuts the tail's tiles by their number and the number of keys alone; a part whose
 // share is empty costs little.  Tiles before the tail run late queries first.
+//
+// One query tile to a CTA up to kShortKeys keys: 512 keys x 3120 queries x 4 rows x 12 heads take 43 us so, 55 in pairs;
+// 14040 keys take 676 us in pairs, and the L2 cannot feed the single tiles' K/V.  A part has at least two key tiles where
+// everything fits one wave (1001 tokens x 3 heads: 20.5 us against 22.5 with four; 256 queries over 1536 keys 22.5 against
+// 24.6), else four: the tail then overlaps the waves before it, and merging two parts of two tiles each costs more than
+// it saves (the 512 keys above: 43.4 against 47.5 us).
 int plan_spans(AttnXParams& p, int sms) {
-  constexpr int kMinTiles = 4;
   constexpr int kShortKeys = 1024;
   p.tiles = p.kv_tokens <= kShortKeys || p.q_tokens <= 128 ? 1 : 2;
   p.pair_tiles = (p.q_tokens + 128 * p.tiles - 1) / (128 * p.tiles);
@@ -832,7 +837,8 @@ int plan_spans(AttnXParams& p, int sms) {
   p.n_tiles = static_cast<int>(n_tiles);
   const int tail = p.n_tiles % wave;
   p.n_full = p.n_tiles - tail;
-  p.split = tail == 0 ? 1 : max(1, min(min(wave / tail, 64), (p.kv_tokens + 127) / 128 / kMinTiles));
+  const int min_tiles = p.n_full == 0 ? 2 : 4;
+  p.split = tail == 0 ? 1 : max(1, min(min(wave / tail, 64), (p.kv_tokens + 127) / 128 / min_tiles));
   p.n_parts = tail * p.split;
   return p.split > 1 ? p.n_parts : 0;
 }
