@@ -604,8 +604,13 @@ static void set_partials(sdv2::AttnXParams& p, void* scratch, int slots) {
 // from four pairs of query tiles on (more than 768 queries) the cache is expanded first, a group of heads at a time so
 // that the scratch stays near 1 GiB.
 //
-// Up to kFewQueries queries have a kernel of their own that never leaves the cache's bytes for shared-memory tiles.
-constexpr int kFewQueries = 32;
+// Up to kFewQueries queries have a kernel of their own that never leaves the cache's bytes for shared-memory tiles: at
+// 32760 keys x 12 heads 50 us for 32 queries (two blocks' worth) against 66 here for 33, at four such rows 160 against 190.
+//
+// A part of a split tile has at least kMinPart tiles of 128 keys: with four, 128 queries over 4000 keys x 12 heads take 23 us,
+// with eight 29, with two 29 (the parts' merging); the kernel of a few queries merges faster and gains down to two (one
+// token over 4000 keys x 2 heads 12 us, 13.5 with four, 17 with eight).
+constexpr int kFewQueries = 32, kMinPart = 4, kFewMinPart = 2;
 struct Q8Run {
   sdv2::AttnXParams p;  // of one head group when expanding first
   bool few;
@@ -642,7 +647,7 @@ static int plan_q8(Q8Run& r, int heads) {
   sdv2::DeviceInfo di;
   const cudaError_t e = sdv2::device_info(&di);
   if (e != cudaSuccess) return cuda_fail(e);
-  const int wave = r.few ? di.sms * sdv2::kFewBlocksPerSm : di.sms, min_tiles = r.few ? 2 : 8;
+  const int wave = r.few ? di.sms * sdv2::kFewBlocksPerSm : di.sms, min_tiles = r.few ? kFewMinPart : kMinPart;
   int last = 0;
   if (heads % r.group != 0) {  // a smaller last group
     r.p.heads = heads % r.group;
@@ -716,7 +721,7 @@ int sdv2_attn_kvcache_q8(const sdv2_view* q, const sdv2_view* k_cache, const sdv
       sdv2::DeviceInfo di;
       if ((e = sdv2::device_info(&di)) != cudaSuccess) return cuda_fail(e);
       r.p.heads = n;
-      if (sdv2::plan_lens(r.p, di.sms, 8) < 0) return SDV2_ERR_UNSUPPORTED_SHAPE;
+      if (sdv2::plan_lens(r.p, di.sms, kMinPart) < 0) return SDV2_ERR_UNSUPPORTED_SHAPE;
     }
     if ((rc = make_tile_map(&tm_q, &qg, rows, q_tokens, n)) != SDV2_OK) return rc;
     if ((rc = make_tile_map(&tm_k, &kx, rows, r.longest, n)) != SDV2_OK) return rc;

@@ -822,14 +822,16 @@ cudaError_t launch_attn_spans(const CUtensorMap& tm_q, const CUtensorMap& tm_k, 
 // Spans live on the device, so the host cuts the tail's tiles by their number and the number of keys alone; a part whose
 // share is empty costs little.  Tiles before the tail run late queries first.
 //
-// One query tile to a CTA up to kShortKeys keys: 512 keys x 3120 queries x 4 rows x 12 heads take 43 us so, 55 in pairs;
-// 14040 keys take 676 us in pairs, and the L2 cannot feed the single tiles' K/V.  A part has at least two key tiles where
+// One query tile to a CTA up to kShortKeys keys, two beyond (3120 queries, microseconds with one and with two): 300 keys
+// x 12 heads 23.2 and 25.2, 512 x 48 heads 60.5 and 65, 1024 x 24 heads 57.8 and 60.2; 2048 x 24 heads 91.6 and 89.2, 4680 x
+// 12 heads 155 and 148.  That holds for 128 queries too, whose second tile is empty: its ring is deeper (12 heads x
+// 16384 keys 66 and 48).  A part has at least two key tiles where
 // everything fits one wave (1001 tokens x 3 heads: 20.5 us against 22.5 with four; 256 queries over 1536 keys 22.5 against
 // 24.6), else four: the tail then overlaps the waves before it, and merging two parts of two tiles each costs more than
 // it saves (the 512 keys above: 43.4 against 47.5 us).
 int plan_spans(AttnXParams& p, int sms) {
   constexpr int kShortKeys = 1024;
-  p.tiles = p.kv_tokens <= kShortKeys || p.q_tokens <= 128 ? 1 : 2;
+  p.tiles = p.kv_tokens <= kShortKeys ? 1 : 2;
   p.pair_tiles = (p.q_tokens + 128 * p.tiles - 1) / (128 * p.tiles);
   const int wave = p.tiles == 1 ? 2 * sms : sms;
   const int64_t n_tiles = static_cast<int64_t>(p.pair_tiles) * p.heads * p.rows;
