@@ -15,8 +15,8 @@ __device__ __forceinline__ void rope_pair(double a, double b, double2 cs, float&
   im = __double2float_rn(__dadd_rn(__dmul_rn(a, cs.y), __dmul_rn(b, cs.x)));
 }
 
-// n / d for n * d < 2^32 with m = ceil(2^32 / d)
-__device__ __forceinline__ int fast_div(uint32_t n, uint32_t m) { return static_cast<int>(__umulhi(n, m)); }
+// n / d for n * d < 2^32 with m = ceil(2^32 / d), which is 0 in 32 bits for d = 1
+__device__ __forceinline__ int fast_div(uint32_t n, uint32_t m) { return static_cast<int>(m == 0 ? n : __umulhi(n, m)); }
 
 // table entry for complex column `col` of a token at (time row, grid row y, grid column x)
 __device__ __forceinline__ double2 table_entry(const AppendParams& p, int col, int64_t trow, int y, int x) {

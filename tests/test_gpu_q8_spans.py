@@ -78,6 +78,24 @@ def test_append_writes_the_format_bit_for_bit(dtype, rows, heads, grid, frames, 
     ops.read_status(torch.device(DEV))
 
 
+@pytest.mark.parametrize("grid", [(3, 1, 1), (2, 5, 1), (1, 7, 1), (2, 1, 6), (3, 4, 1)])
+def test_appends_of_grids_one_token_wide_or_high(grid):
+    """Frames, rows and columns of one: the 8-bit append against its statement, and the plain append's keys and queries
+    against the 64-bit rope rounded once."""
+    n = grid[0] * grid[1] * grid[2]
+    q, k, v = (_randn(s, 2, n, 3, 128) for s in (1, 2, 3))
+    c = _garbage_cache(2, n + 9, 3)
+    want = _expected(c, k, v, grid, [5, 100], [4, 0])
+    d = _cuda(c)
+    q_out = _append(d, q.to(DEV), k.to(DEV), v.to(DEV), grid, [5, 100], [4, 0])
+    _same_cache(d, want)
+    kc = torch.zeros(2, n, 3, 128, device=DEV)
+    vc = torch.zeros_like(kc)
+    q_plain = _ops().rope_kv_append(q.to(DEV), k.to(DEV), v.to(DEV), kc, vc, _table().to(DEV), grid, [5, 100], [0, 0])
+    assert torch.equal(kc.cpu(), ref.rope64(k, _table(), grid, [5, 100]).float()) and torch.equal(vc.cpu(), v)
+    assert torch.equal(q_out, q_plain) and torch.equal(q_out.cpu(), ref.rope64(q, _table(), grid, [5, 100]).float())
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_append_special_values(dtype):
     """Zeros, subnormals, the largest finite values, infinities and NaN, values on rounding ties and above 127.5 steps."""
