@@ -554,8 +554,13 @@ attn_x_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
             attended = (static_cast<uint32_t>(bits[row >> 5]) >> (row & 31)) & 1u;
             ++n_mixed;
           }
-          ok = kTiles == 1 ? mbar_wait(bar(kBarVFull), j & 1, abort_flag, p.status, WAIT_KV_FULL)
-                           : mbar_wait(bar(kBarPairFull + j % kPairBars), (j / kPairBars) & 1, abort_flag, p.status, WAIT_KV_FULL);
+          // With one V slot the barrier's phase says only whether tile j or j - 1 is the last to have arrived, and tile j - 1
+          // may still be on its way if it was not a mixed one.  S_j is issued behind P V of tile j - 1, so it settles that;
+          // with three pair barriers pair j - 3 has long arrived.
+          if (kTiles == 1) ok = mbar_wait(bar(kBarSFull), j & 1, abort_flag, p.status, WAIT_S_FULL);
+          ok = ok && (kTiles == 1 ? mbar_wait(bar(kBarVFull), j & 1, abort_flag, p.status, WAIT_KV_FULL)
+                                  : mbar_wait(bar(kBarPairFull + j % kPairBars), (j / kPairBars) & 1, abort_flag, p.status,
+                                              WAIT_KV_FULL));
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           if (!attended) {

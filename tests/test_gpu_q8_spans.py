@@ -512,6 +512,22 @@ def test_spans_attention_heads_outermost_and_offsets_past_32_bits(n, S):
     del big, kd, vd
 
 
+@pytest.mark.parametrize("rows,n,heads,S", [(24, 2, 26, 994), (3, 300, 5, 900), (8, 130, 20, 1000), (2, 700, 5, 3000)])
+def test_spans_attention_gives_the_same_bits_whatever_the_timing(rows, n, heads, S):
+    """Fresh operands (nothing cached) and then the same again: tiles that a span covers next to tiles that it cuts, whose
+    keys arrive late in the first call."""
+    ops = _ops()
+    g = torch.Generator(DEV).manual_seed(3)
+    flush = torch.empty(1 << 26, device=DEV)
+    for _ in range(40):
+        q, k, v = (torch.randn(rows, m, heads, 128, generator=g, device=DEV).to(torch.bfloat16) for m in (n, S, S))
+        a, b = (torch.randint(-5, S + 6, (rows, n), generator=g, device=DEV, dtype=torch.int32) for _ in range(2))
+        a, b = torch.minimum(a, b), torch.maximum(a, b)
+        flush.fill_(1.0)
+        first, second, third = (ops.attn_spans(q, k, v, a, b) for _ in range(3))
+        assert torch.equal(first, second) and torch.equal(second, third)
+
+
 def test_span_attention_over_whole_rows_agrees_with_the_cache_kernel():
     ops = _ops()
     q, k, v = (_randn(s, 2, m, 3, 128).to(torch.bfloat16).to(DEV) for s, m in ((1, 500), (2, 900), (3, 900)))
