@@ -16,6 +16,11 @@
 //   of the CTA attends are cleared on chip (0 x NaN would reach the output otherwise).  Rows with an empty span give 0.
 //
 // Split tiles write unnormalised O, the running maximum, sum and V exponent to scratch; combine_kernel merges them.
+//
+// Bound by the chain S -> softmax -> P V of a query tile, two of which share the tensor pipe and the exp unit (both some
+// 60 % busy): 3800 cycles a step of 128 keys for 256 queries.  14040 queries in three blocks over 14040 keys x 12 heads:
+// 664-676 us, 1.2 PFLOP/s (782 us in long runs under the power cap); 2 x 3120 queries over 32760 expanded keys x 12 heads 1.0
+// ms of 1.1; expanded here, 256 queries over 32760 keys x 12 heads 75 us.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
