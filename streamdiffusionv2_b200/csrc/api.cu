@@ -612,6 +612,7 @@ static void set_partials(sdv2::AttnXParams& p, void* scratch, int slots) {
 // with eight 29, with two 29 (the parts' merging); the kernel of a few queries merges faster and gains down to two (one
 // token over 4000 keys x 2 heads 12 us, 13.5 with four, 17 with eight).
 constexpr int kFewQueries = 32, kMinPart = 4, kFewMinPart = 2;
+constexpr int kSetup = 2, kFewSetup = 4;  // set-up, first loads and epilogue in key tiles' time (6000 to 3800 cycles; 15000 to 4200)
 struct Q8Run {
   sdv2::AttnXParams p;  // of one head group when expanding first
   bool few;
@@ -649,13 +650,14 @@ static int plan_q8(Q8Run& r, int heads) {
   const cudaError_t e = sdv2::device_info(&di);
   if (e != cudaSuccess) return cuda_fail(e);
   const int wave = r.few ? di.sms * sdv2::kFewBlocksPerSm : di.sms, min_tiles = r.few ? kFewMinPart : kMinPart;
+  const int setup = r.few ? kFewSetup : kSetup;
   int last = 0;
   if (heads % r.group != 0) {  // a smaller last group
     r.p.heads = heads % r.group;
-    last = sdv2::plan_lens(r.p, wave, min_tiles);
+    last = sdv2::plan_lens(r.p, wave, min_tiles, setup);
   }
   r.p.heads = r.group;
-  r.slots = sdv2::plan_lens(r.p, wave, min_tiles);
+  r.slots = sdv2::plan_lens(r.p, wave, min_tiles, setup);
   if (r.slots < 0 || last < 0) return SDV2_ERR_UNSUPPORTED_SHAPE;
   if (last > r.slots) r.slots = last;
   return SDV2_OK;
@@ -722,7 +724,7 @@ int sdv2_attn_kvcache_q8(const sdv2_view* q, const sdv2_view* k_cache, const sdv
       sdv2::DeviceInfo di;
       if ((e = sdv2::device_info(&di)) != cudaSuccess) return cuda_fail(e);
       r.p.heads = n;
-      if (sdv2::plan_lens(r.p, di.sms, kMinPart) < 0) return SDV2_ERR_UNSUPPORTED_SHAPE;
+      if (sdv2::plan_lens(r.p, di.sms, kMinPart, kSetup) < 0) return SDV2_ERR_UNSUPPORTED_SHAPE;
     }
     if ((rc = make_tile_map(&tm_q, &qg, rows, q_tokens, n)) != SDV2_OK) return rc;
     if ((rc = make_tile_map(&tm_k, &kx, rows, r.longest, n)) != SDV2_OK) return rc;

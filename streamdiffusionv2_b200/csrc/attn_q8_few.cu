@@ -24,6 +24,8 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <algorithm>
+
 #include "attn_items.cuh"
 #include "ptx.cuh"
 #include "q8.cuh"
@@ -484,10 +486,13 @@ cudaError_t launch_attn_few(const CUtensorMap& tm_k, const CUtensorMap& tm_v, co
 }
 
 // Splitting along the keys.  With `wave` CTAs on the GPU at a time, n_tiles = waves * wave + tail leaves only `tail` of
-// those places busy at the end (all of them, when there are few tiles).  The tail's tiles - those of the shortest rows,
-// rows are taken longest first - are cut into parts of about c tiles of 128 keys, c the smallest for which the parts
-// still fit one wave.  A part costs its set-up and a pass over its accumulator, so c stays at min_tiles or more.
-int plan_lens(AttnXParams& p, int wave, int min_tiles) {
+// those places busy at the end (all of them, when there are few tiles).  Rows are taken longest first, and the tail's tiles
+// are cut into parts of about c tiles of 128 keys, c the smallest for which the parts fit the places: short items
+// share one as far as they end with the others (an item costs `setup` key tiles beside its own).  A part costs its set-up
+// and a pass over its accumulator, so c stays at min_tiles or more.  Rows so long that a tile of theirs would outlast all
+// else (twice a place's share) belong to the tail whole: one row of 32760 keys among fifteen of 100 x 40 heads would
+// keep 40 places busy and leave 400 idle (one token: 234 us, cut up 67).
+int plan_lens(AttnXParams& p, int wave, int min_tiles, int setup) {
   const int per_row = p.pair_tiles * p.heads;
   int n_kv[SDV2_MAX_ROWS], first[SDV2_MAX_ROWS];
   for (int r = 1; r < p.rows; ++r) {  // insertion sort, longest row first
@@ -499,7 +504,15 @@ int plan_lens(AttnXParams& p, int wave, int min_tiles) {
   const int64_t n_tiles = static_cast<int64_t>(per_row) * p.rows;
   if (n_tiles > 0x7FFFFFFFLL / 64) return -1;
   p.n_tiles = static_cast<int>(n_tiles);
-  p.n_full = p.n_tiles - p.n_tiles % wave;
+  int n_long = 0;
+  if (p.n_tiles >= wave) {
+    int64_t work = 0;
+    for (int r = 0; r < p.rows; ++r) work += static_cast<int64_t>(per_row) * ((p.by_length[r].len + 127) / 128);
+    while (n_long < p.rows && (p.by_length[n_long].len + 127) / 128 > max(2 * work / wave, static_cast<int64_t>(min_tiles))) ++n_long;
+    std::rotate(p.by_length, p.by_length + n_long, p.by_length + p.rows);
+  }
+  const int n_other = p.n_tiles - n_long * per_row;
+  p.n_full = n_other - n_other % wave;
   int longest = 0;
   for (int r = 0; r < p.rows; ++r) {
     n_kv[r] = (p.by_length[r].len + 127) / 128;
@@ -507,15 +520,18 @@ int plan_lens(AttnXParams& p, int wave, int min_tiles) {
     if ((r + 1) * per_row > p.n_full) longest = max(longest, n_kv[r]);
   }
   auto parts_at = [&](int c, int r) { return n_kv[r] <= c ? 1 : (n_kv[r] + c - 1) / c; };
-  auto items_at = [&](int c) {
-    int64_t n = 0;
-    for (int r = 0; r < p.rows; ++r) n += static_cast<int64_t>(max((r + 1) * per_row - first[r], 0)) * parts_at(c, r);
+  auto places_at = [&](int c) {
+    double n = 0.;
+    for (int r = 0; r < p.rows; ++r) {
+      const int parts = parts_at(c, r);
+      n += static_cast<double>(max((r + 1) * per_row - first[r], 0)) * parts / ((c + setup) / ((n_kv[r] + parts - 1) / parts + setup));
+    }
     return n;
   };
-  int lo = min_tiles, hi = max(longest, min_tiles);  // the smallest c in [lo, hi] whose parts fit; hi always does
+  int lo = min_tiles, hi = max(longest, min_tiles);  // the smallest c in [lo, hi] whose parts fit, else hi
   while (lo < hi) {
     const int c = (lo + hi) / 2;
-    if (items_at(c) <= wave) hi = c;
+    if (places_at(c) <= wave) hi = c;
     else lo = c + 1;
   }
   p.split = 1;

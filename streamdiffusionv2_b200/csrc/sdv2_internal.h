@@ -209,7 +209,7 @@ struct AttnXParams {
   // 8-bit cache, lengths: rows longest first, parts[r] parts for the tiles of a row
   sdv2_view q, k, v, k_exp, v_exp;
   int k_row_mask, v_row_mask;      // 0: every row reads row 0 of K / V, else all ones
-  // longest row first; what a CTA needs of its row lies together (a line of the parameter bank costs some 400 cycles)
+  // longest row first, then very long ones; what a CTA needs of its row lies together (a line of the parameter bank costs some 400 cycles)
   struct Row {
     int row, len;
     int tail_tile0, item0, parts;  // first of its tail tiles, first of their items, items of each
@@ -221,7 +221,7 @@ struct AttnXParams {
 };
 constexpr size_t kAttnXPartFloats = 128 * 128 + 3 * 128;  // of one query tile
 // Fill in how the work is cut up; returns the partial-result slots needed (0: none) or -1 (too many tiles).
-int plan_lens(AttnXParams& p, int wave, int min_tiles);
+int plan_lens(AttnXParams& p, int wave, int min_tiles, int setup);
 int plan_spans(AttnXParams& p, int sms);
 constexpr int kFewRows = 16;        // most query rows of a block of launch_attn_few; partials: [parts][16][128], [parts][2][16]
 constexpr int kFewBlocksPerSm = 3;

@@ -287,6 +287,19 @@ def test_q8_attention_ignores_junk_behind_the_length_and_in_scratch(queries):
     _check_q8(c, q, lens, out)
 
 
+@pytest.mark.parametrize("queries,heads,lens", [
+    (1, 40, [3000] + [100] * 15), (20, 30, [5, 2900, 0, 1, 260, 3000] + [64] * 8), (130, 12, [70, 3000] + [200] * 14),
+    (900, 5, [4000] + [130] * 11),
+])
+def test_q8_attention_rows_far_longer_than_the_others(queries, heads, lens):
+    """More tiles than fit the GPU at a time: the long rows are cut up, the others run whole."""
+    ops = _ops()
+    c = _held_cache(len(lens), max(lens), heads, 12, spread=1.0)
+    q = _randn(5, len(lens), queries, heads, 128).to(torch.bfloat16)
+    d = _cuda(c)
+    _check_q8(c, q, lens, ops.attn_kvcache_q8(q.to(DEV), d["k"], d["v"], d["k_exp"], d["v_exp"], lens))
+
+
 def test_q8_attention_in_groups_of_heads():
     """Many queries over a cache too large to expand at once: 23 heads in groups of 12 and 11, one row nearly empty."""
     ops = _ops()
