@@ -740,57 +740,89 @@ attn_x_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
   }
 }
 
-// Merge the parts of the split tiles.  Block = (split tile, query tile, group of 32 rows); 256 threads = 32 rows x 8
-// column groups of 16.  out = sum_k w_k O_k / sum_k 2^(m_k - m) l_k with w_k = 2^(m_k - m + R_k - R) and the result in
-// units of 2^(R+6); a part without a key has l_k = 0 and no accumulator.
+// Merge the parts of the split tiles.  Block = (split tile, query tile, group of 8 rows), a warp a row, a lane four dims.
+// out = sum_k w_k O_k / sum_k 2^(m_k - m) l_k with w_k = 2^(m_k - m + R_k - R) and the result in units of 2^(R+6); a part
+// without a key has l_k = 0 and no accumulator (what lies in its place is not used).  Bound by the latency of its loads: the
+// first kAhead parts' are made before the weights are known, and a lane has the weights of every 32nd part.
+constexpr int kMergeRows = 8;
 template <int kMode, int kTiles>
-__global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ AttnXParams p) {
+__global__ void __launch_bounds__(kMergeRows * 32) combine_kernel(const __grid_constant__ AttnXParams p) {
   constexpr bool kQ8 = kMode == kModeExpand, kSpans = kMode == kModeSpans;
-  const int stage = blockIdx.y;
-  const int row = blockIdx.z * 32 + (threadIdx.x >> 3);
-  const int c0 = (threadIdx.x & 7) * 16;
+  constexpr int kAhead = 8;
+  const int stage = blockIdx.y, lane = threadIdx.x & 31;
+  const int row = blockIdx.z * kMergeRows + (threadIdx.x >> 5);
   const Item item =
       find_item<kSpans>(p, kSpans ? p.n_full + static_cast<int>(blockIdx.x) * p.split : first_item_lens(p, blockIdx.x));
   const int q_row = item.tile * (kTiles * kBM) + stage * kBM + row;
   asm volatile("griddepcontrol.wait;" ::: "memory");  // the parts are complete
   if (item.part < 0 || q_row >= p.q_tokens) return;
   const float* pm = p.part_meta + (static_cast<size_t>(item.slot) * kTiles + stage) * (3 * kBM) + row;
-  const float* po = p.part_o + (static_cast<size_t>(item.slot) * kTiles + stage) * (kBM * kHD) + row * kHD + c0;
+  const float* po = p.part_o + (static_cast<size_t>(item.slot) * kTiles + stage) * (kBM * kHD) + row * kHD + lane * 4;
   constexpr size_t pm_step = kTiles * 3 * kBM, po_step = static_cast<size_t>(kTiles) * kBM * kHD;
-  float m = -INFINITY, ref = q8::kMinExp;
-  for (int k = 0; k < item.parts; ++k) {
+  float4 a[kAhead];
+  auto load = [&](int k0) {
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+      if (k0 + i < item.parts) a[i] = *reinterpret_cast<const float4*>(po + (k0 + i) * po_step);
+  };
+  load(0);
+  float mk[2], lk[2], rk[2];  // of parts lane, lane + 32; later ones (few queries' worth of tiles) are read again
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int k = lane + 32 * i;
+    mk[i] = k < item.parts ? pm[k * pm_step] : -INFINITY;
+    lk[i] = k < item.parts ? pm[k * pm_step + kBM] : 0.f;
+    rk[i] = kQ8 && lk[i] != 0.f ? pm[k * pm_step + 2 * kBM] : q8::kMinExp;
+  }
+  float m = fmaxf(mk[0], mk[1]), ref = fmaxf(rk[0], rk[1]);
+  for (int k = 64 + lane; k < item.parts; k += 32) {
     m = fmaxf(m, pm[k * pm_step]);
     if (kQ8 && pm[k * pm_step + kBM] != 0.f) ref = fmaxf(ref, pm[k * pm_step + 2 * kBM]);
   }
+#pragma unroll
+  for (int i = 16; i > 0; i >>= 1) {
+    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, i));
+    if (kQ8) ref = fmaxf(ref, __shfl_xor_sync(0xffffffffu, ref, i));
+  }
   const float m_sub = m == -INFINITY ? 0.f : m;
-  float l = 0.f;
-  float acc[16];
+  auto shift = [&](float r) { return kQ8 ? exp2_int(static_cast<int>(r - ref)) : 1.f; };
+  float wk[2], l = 0.f;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) acc[i] = 0.f;
-  for (int k = 0; k < item.parts; ++k) {
-    const float lk = pm[k * pm_step + kBM];
-    if (lk == 0.f) continue;
-    const float up = exp2f(pm[k * pm_step] - m_sub);
-    const float w = kQ8 ? up * exp2_int(static_cast<int>(pm[k * pm_step + 2 * kBM] - ref)) : up;
-    l += up * lk;
+  for (int i = 0; i < 2; ++i) {
+    const float up = lk[i] == 0.f ? 0.f : exp2f(mk[i] - m_sub);
+    l += up * lk[i];
+    wk[i] = up * shift(rk[i]);
+  }
+  for (int k = 64 + lane; k < item.parts; k += 32)
+    if (pm[k * pm_step + kBM] != 0.f) l += exp2f(pm[k * pm_step] - m_sub) * pm[k * pm_step + kBM];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float4 a = *reinterpret_cast<const float4*>(po + k * po_step + 4 * i);
-      acc[4 * i + 0] += w * a.x; acc[4 * i + 1] += w * a.y; acc[4 * i + 2] += w * a.z; acc[4 * i + 3] += w * a.w;
+  for (int i = 16; i > 0; i >>= 1) l += __shfl_xor_sync(0xffffffffu, l, i);
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int k0 = 0; k0 < item.parts; k0 += kAhead) {
+    if (k0 > 0) load(k0);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int k = k0 + i;
+      if (k >= item.parts) break;
+      float w, lp;
+      if (k < 64) {
+        w = __shfl_sync(0xffffffffu, k < 32 ? wk[0] : wk[1], k & 31);
+        lp = __shfl_sync(0xffffffffu, k < 32 ? lk[0] : lk[1], k & 31);
+      } else {
+        w = exp2f(pm[k * pm_step] - m_sub) * shift(pm[k * pm_step + 2 * kBM]);
+        lp = pm[k * pm_step + kBM];
+      }
+      if (lp == 0.f) continue;
+      acc.x += w * a[i].x; acc.y += w * a[i].y; acc.z += w * a[i].z; acc.w += w * a[i].w;
     }
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
   const float unit = kQ8 ? exp2_int(static_cast<int>(ref) + 6) : 1.f;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) acc[i] = acc[i] * inv * unit;
   __nv_bfloat16* op = static_cast<__nv_bfloat16*>(p.out) + static_cast<int64_t>(item.b) * p.out_stride_row +
                       static_cast<int64_t>(q_row) * p.out_stride_tok +
-                      static_cast<int64_t>(item.h) * p.out_stride_head + c0;
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-    *reinterpret_cast<uint4*>(op + 8 * i) =
-        make_uint4(pack_bf16x2(acc[8 * i + 0], acc[8 * i + 1]), pack_bf16x2(acc[8 * i + 2], acc[8 * i + 3]),
-                   pack_bf16x2(acc[8 * i + 4], acc[8 * i + 5]), pack_bf16x2(acc[8 * i + 6], acc[8 * i + 7]));
+                      static_cast<int64_t>(item.h) * p.out_stride_head + lane * 4;
+  *reinterpret_cast<uint2*>(op) =
+      make_uint2(pack_bf16x2(acc.x * inv * unit, acc.y * inv * unit), pack_bf16x2(acc.z * inv * unit, acc.w * inv * unit));
 }
 
 template <int kMode, int kTiles>
@@ -808,8 +840,8 @@ cudaError_t launch(const CUtensorMap& tm_q, const CUtensorMap& tm_k, const CUten
                      Shape<kMode, kTiles>::kSmemBytes, stream, kMode == kModeLens, tm_q, tm_k, tm_v, p);
   if (e != cudaSuccess || p.split == 1) return e;
   const int merged = p.n_tiles - p.n_full;
-  return launch_chained(combine_kernel<kMode, kTiles>, dim3(merged, kTiles == 2 && p.q_tokens > kBM ? 2 : 1, kBM / 32), dim3(256),
-                        0, stream, true, p);
+  return launch_chained(combine_kernel<kMode, kTiles>, dim3(merged, kTiles == 2 && p.q_tokens > kBM ? 2 : 1, kBM / kMergeRows),
+                        dim3(kMergeRows * 32), 0, stream, true, p);
 }
 
 }  // namespace attnx
