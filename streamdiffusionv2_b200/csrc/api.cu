@@ -606,12 +606,11 @@ static void set_partials(sdv2::AttnXParams& p, void* scratch, int slots) {
 // expanding first, 800 queries 216 and 221, over 2 rows x 9000 keys x 40 heads 411 and 396.
 //
 // Up to kFewQueries queries have a kernel of their own that never leaves the cache's bytes for shared-memory tiles: at
-// 32760 keys x 12 heads 50 us for 32 queries (two blocks' worth) against 66 here for 33, at four such rows 160 against 190.
+// 32760 keys x 12 heads 50 us for 32 queries (two blocks' worth) against 61 here for 33, at four such rows 160 against 187.
 //
-// A part of a split tile has at least kMinPart tiles of 128 keys: with four, 128 queries over 4000 keys x 12 heads take 23 us,
-// with eight 29, with two 29 (the parts' merging); the kernel of a few queries merges faster and gains down to two (one
-// token over 4000 keys x 2 heads 12 us, 13.5 with four, 17 with eight).
-constexpr int kFewQueries = 32, kMinPart = 4, kFewMinPart = 2;
+// A part of a split tile has at least kMinPart tiles of 128 keys: with two, 200 queries over 4000 keys x 2 heads take 19 us,
+// with four 23, with eight 31; one token over them 12 us, 13.5 and 17.
+constexpr int kFewQueries = 32, kMinPart = 2;
 constexpr int kSetup = 2, kFewSetup = 4;  // set-up, first loads and epilogue in key tiles' time (6000 to 3800 cycles; 15000 to 4200)
 struct Q8Run {
   sdv2::AttnXParams p;  // of one head group when expanding first
@@ -649,15 +648,15 @@ static int plan_q8(Q8Run& r, int heads) {
   sdv2::DeviceInfo di;
   const cudaError_t e = sdv2::device_info(&di);
   if (e != cudaSuccess) return cuda_fail(e);
-  const int wave = r.few ? di.sms * sdv2::kFewBlocksPerSm : di.sms, min_tiles = r.few ? kFewMinPart : kMinPart;
+  const int wave = r.few ? di.sms * sdv2::kFewBlocksPerSm : di.sms;
   const int setup = r.few ? kFewSetup : kSetup;
   int last = 0;
   if (heads % r.group != 0) {  // a smaller last group
     r.p.heads = heads % r.group;
-    last = sdv2::plan_lens(r.p, wave, min_tiles, setup);
+    last = sdv2::plan_lens(r.p, wave, kMinPart, setup);
   }
   r.p.heads = r.group;
-  r.slots = sdv2::plan_lens(r.p, wave, min_tiles, setup);
+  r.slots = sdv2::plan_lens(r.p, wave, kMinPart, setup);
   if (r.slots < 0 || last < 0) return SDV2_ERR_UNSUPPORTED_SHAPE;
   if (last > r.slots) r.slots = last;
   return SDV2_OK;

@@ -20,7 +20,7 @@
 // Bound by the chain S -> softmax -> P V of a query tile, two of which share the tensor pipe and the exp unit (both some
 // 60 % busy): 3800 cycles a step of 128 keys for 256 queries.  14040 queries in three blocks over 14040 keys x 12 heads:
 // 664-676 us, 1.2 PFLOP/s (782 us in long runs under the power cap); 2 x 3120 queries over 32760 expanded keys x 12 heads 1.0
-// ms of 1.1; expanded here, 256 queries over 32760 keys x 12 heads 75 us.
+// ms of 1.1; expanded here, 256 queries over 32760 keys x 12 heads 71 us.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -869,7 +869,7 @@ cudaError_t launch_attn_spans(const CUtensorMap& tm_q, const CUtensorMap& tm_k, 
 // 12 heads 155 and 148.  That holds for 128 queries too, whose second tile is empty: its ring is deeper (12 heads x
 // 16384 keys 66 and 48).  A part has at least two key tiles where
 // everything fits one wave (1001 tokens x 3 heads: 20.5 us against 22.5 with four; 256 queries over 1536 keys 22.5 against
-// 24.6), else four: the tail then overlaps the waves before it, and merging two parts of two tiles each costs more than
+// 24.6; both 18.4 with today's merging), else four: the tail then overlaps the waves before it, and merging two parts of two tiles each costs more than
 // it saves (the 512 keys above: 43.4 against 47.5 us).
 int plan_spans(AttnXParams& p, int sms) {
   constexpr int kShortKeys = 1024;
