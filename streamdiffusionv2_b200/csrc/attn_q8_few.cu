@@ -99,7 +99,6 @@ attn_few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
     fence_mbar_init();
   }
   __syncwarp();
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the merging kernel may be set up meanwhile
   const Item item = attnx::find_item_lens(p, blockIdx.x);
   const int b = item.b, h = item.h, q0 = item.tile * kRows;
   const int n_all = (item.len + 127) / 128;
@@ -124,6 +123,7 @@ attn_few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
     next_k = keb[key * p.k_exp.stride_tok];
     next_v = veb[key * p.v_exp.stride_tok];
   };
+  begin_after_previous_kernel();
   load(0, first0);
 
   // query fragments: k-step hf * 4 + w holds dims hf * 64 + t4 * 16 + w * 4 + {0, 1} and {2, 3} of query g
@@ -408,7 +408,7 @@ __global__ void __launch_bounds__(256) combine_few_kernel(const __grid_constant_
   const int row = blockIdx.y, lane = threadIdx.x & 31, c0 = lane * 4, grp = threadIdx.x >> 5;
   const Item item = attnx::find_item_lens(p, attnx::first_item_lens(p, blockIdx.x));
   const int q_row = item.tile * p.few_rows + row;
-  asm volatile("griddepcontrol.wait;" ::: "memory");  // the parts are complete
+  begin_after_previous_kernel();  // the parts are complete
   if (item.part < 0 || q_row >= p.q_tokens) return;
   const float* pm = p.part_meta + static_cast<size_t>(item.slot) * 2 * kFewRows + row;
   const float* po = p.part_o + (static_cast<size_t>(item.slot) * kFewRows + row) * 128 + c0;
@@ -473,10 +473,9 @@ cudaError_t launch(const CUtensorMap& tm_k, const CUtensorMap& tm_v, const AttnX
   cudaError_t e = device_info(&di);
   if (e == cudaSuccess) e = smem_grant.ensure(attn_few_kernel<kN>, kSmemBytes, di.device);
   if (e != cudaSuccess) return e;
-  attn_few_kernel<kN><<<p.n_full + p.n_parts, kWarps * 32, kSmemBytes, stream>>>(tm_k, tm_v, p);
-  e = cudaGetLastError();
+  e = launch_chained(attn_few_kernel<kN>, dim3(p.n_full + p.n_parts), dim3(kWarps * 32), kSmemBytes, stream, tm_k, tm_v, p);
   if (e != cudaSuccess || p.split == 1) return e;
-  return launch_chained(combine_few_kernel, dim3(p.n_tiles - p.n_full, min(p.q_tokens, p.few_rows)), dim3(256), 0, stream, true, p);
+  return launch_chained(combine_few_kernel, dim3(p.n_tiles - p.n_full, min(p.q_tokens, p.few_rows)), dim3(256), 0, stream, p);
 }
 
 }  // namespace few

@@ -252,11 +252,7 @@ attn_x_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
       mbar_init(bar(kBarOFull + i), 1);
     }
     fence_mbar_init();
-    for (int s = 0; s < n_stage; ++s) {  // the queries are wanted whatever the keys; the issuing thread waits for them
-      mbar_expect_tx(bar(kBarQFull + s), kTileBytes);
-      tma_load_4d(base + s * kTileBytes, &tm_q, bar(kBarQFull + s), 0, h, q0 + s * kBM, b);
-      tma_load_4d(base + s * kTileBytes + kHalfTile, &tm_q, bar(kBarQFull + s), 64, h, q0 + s * kBM, b);
-    }
+    tma_prefetch_desc(&tm_q);
     if (!kQ8) {
       tma_prefetch_desc(&tm_k);
       tma_prefetch_desc(&tm_v);
@@ -266,7 +262,14 @@ attn_x_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
     tmem_alloc(smem_u32(const_cast<int*>(words + kWordTmem)), Sh::kTmemCols);
     tmem_relinquish();
   }
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the merging kernel may be set up meanwhile
+  begin_after_previous_kernel();
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < n_stage; ++s) {  // the queries are wanted whatever the keys; the issuing thread waits for them
+      mbar_expect_tx(bar(kBarQFull + s), kTileBytes);
+      tma_load_4d(base + s * kTileBytes, &tm_q, bar(kBarQFull + s), 0, h, q0 + s * kBM, b);
+      tma_load_4d(base + s * kTileBytes + kHalfTile, &tm_q, bar(kBarQFull + s), 64, h, q0 + s * kBM, b);
+    }
+  }
   // this thread's query row (softmax warps) and its span, clipped to the keys there are; for the threads of query tile 0
   // that of the row 128 further on too
   constexpr int kSoftmaxWarp0 = Sh::kSoftmaxWarp0;
@@ -455,7 +458,6 @@ attn_x_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
         tma_load_4d(base + slot_off(it), tm, full_bar, 0, h, (j0 + kv_tile) * kBN, bk);
         tma_load_4d(base + slot_off(it) + kHalfTile, tm, full_bar, 64, h, (j0 + kv_tile) * kBN, bk);
       };
-      if (kMode == kModeLens) asm volatile("griddepcontrol.wait;" ::: "memory");  // the keys and values are expanded
       mbar_expect_tx(bar(kBarK0Full), kTileBytes);
       load_tile(&tm_k, 0, 0, bar(kBarK0Full));
       bool ok = true;
@@ -754,7 +756,7 @@ __global__ void __launch_bounds__(kMergeRows * 32) combine_kernel(const __grid_c
   const Item item =
       find_item<kSpans>(p, kSpans ? p.n_full + static_cast<int>(blockIdx.x) * p.split : first_item_lens(p, blockIdx.x));
   const int q_row = item.tile * (kTiles * kBM) + stage * kBM + row;
-  asm volatile("griddepcontrol.wait;" ::: "memory");  // the parts are complete
+  begin_after_previous_kernel();  // the parts are complete
   if (item.part < 0 || q_row >= p.q_tokens) return;
   const float* pm = p.part_meta + (static_cast<size_t>(item.slot) * kTiles + stage) * (3 * kBM) + row;
   const float* po = p.part_o + (static_cast<size_t>(item.slot) * kTiles + stage) * (kBM * kHD) + row * kHD + lane * 4;
@@ -835,13 +837,12 @@ cudaError_t launch(const CUtensorMap& tm_q, const CUtensorMap& tm_k, const CUten
   if (e == cudaSuccess) e = smem_grant.ensure(attn_x_kernel<kMode, kTiles>, static_cast<int>(Shape<kMode, kTiles>::kSmemBytes), di.device);
   if (e != cudaSuccess) return e;
   const int items = p.n_full + p.n_parts;
-  // kModeLens follows kv_read_q8_kernel, behind whose last blocks its set-up passes
   e = launch_chained(attn_x_kernel<kMode, kTiles>, dim3(items), dim3(Shape<kMode, kTiles>::kThreads),
-                     Shape<kMode, kTiles>::kSmemBytes, stream, kMode == kModeLens, tm_q, tm_k, tm_v, p);
+                     Shape<kMode, kTiles>::kSmemBytes, stream, tm_q, tm_k, tm_v, p);
   if (e != cudaSuccess || p.split == 1) return e;
   const int merged = p.n_tiles - p.n_full;
   return launch_chained(combine_kernel<kMode, kTiles>, dim3(merged, kTiles == 2 && p.q_tokens > kBM ? 2 : 1, kBM / kMergeRows),
-                        dim3(kMergeRows * 32), 0, stream, true, p);
+                        dim3(kMergeRows * 32), 0, stream, p);
 }
 
 }  // namespace attnx

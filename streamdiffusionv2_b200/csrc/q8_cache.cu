@@ -132,6 +132,7 @@ template <typename T>
 __global__ void __launch_bounds__(kWarpsPerBlock * 32, sizeof(T) == 2 ? 6 : 5)
 rope_kv_append_q8_kernel(const __grid_constant__ Q8AppendParams qp) {
   const AppendParams& p = qp.a;
+  begin_after_previous_kernel();
   if (!step_params_ok(p)) {
     if (blockIdx.x == 0 && threadIdx.x == 0) report_bad_step_params(p);
     return;
@@ -241,7 +242,7 @@ __device__ __forceinline__ void store32(void* p, const uint32_t (&w)[8]) {
 // 6.05 TB/s, bound by HBM; 110 us with two 16-byte stores in their place).
 template <bool kBf16, bool kWide>
 __global__ void __launch_bounds__(256) kv_read_q8_kernel(const __grid_constant__ Q8ReadParams p) {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // an attention that follows may be set up meanwhile
+  begin_after_previous_kernel();
   const int b = blockIdx.y;
   const int t0 = blockIdx.x * p.block_tokens;
   const int n = min(p.block_tokens, p.count[b] - t0) * p.row_vecs;
@@ -323,11 +324,8 @@ cudaError_t launch_rope_kv_append_q8(const Q8AppendParams& p_in, int dtype, cuda
   if (warps > 0x7FFFFF00LL) return cudaErrorInvalidValue;
   const int64_t blocks = (warps + q8::kWarpsPerBlock - 1) / q8::kWarpsPerBlock;
   constexpr int kThreads = q8::kWarpsPerBlock * 32;
-  if (dtype == SDV2_DTYPE_BF16)
-    q8::rope_kv_append_q8_kernel<__nv_bfloat16><<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(p);
-  else
-    q8::rope_kv_append_q8_kernel<float><<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(p);
-  return cudaGetLastError();
+  auto* kernel = dtype == SDV2_DTYPE_BF16 ? q8::rope_kv_append_q8_kernel<__nv_bfloat16> : q8::rope_kv_append_q8_kernel<float>;
+  return launch_chained(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, stream, p);
 }
 
 cudaError_t launch_kv_read_q8(const Q8ReadParams& p_in, cudaStream_t stream) {
@@ -346,8 +344,7 @@ cudaError_t launch_kv_read_q8(const Q8ReadParams& p_in, cudaStream_t stream) {
   const bool w = wide(p.k_out) && wide(p.v_out);
   auto* kernel = p.dtype == SDV2_DTYPE_BF16 ? (w ? q8::kv_read_q8_kernel<true, true> : q8::kv_read_q8_kernel<true, false>)
                                             : (w ? q8::kv_read_q8_kernel<false, true> : q8::kv_read_q8_kernel<false, false>);
-  kernel<<<grid, 256, 0, stream>>>(p);
-  return cudaGetLastError();
+  return launch_chained(kernel, grid, dim3(256), 0, stream, p);
 }
 
 }  // namespace sdv2

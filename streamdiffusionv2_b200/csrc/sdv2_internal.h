@@ -147,10 +147,10 @@ __device__ __forceinline__ uint32_t rms_scale_pair(uint32_t x, float rstd, uint3
 }
 #endif
 
-// Launch `kernel`; with `early` so that its set-up overlaps the end of the kernel before it on the stream, for whose
-// results it then has to wait with griddepcontrol.wait.
+// Launch `kernel` so that its set-up overlaps the end of the kernel before it on the stream, whoever's that is; every
+// thread of it calls begin_after_previous_kernel() before it touches global memory.
 template <typename... Params, typename... Args>
-cudaError_t launch_chained(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem_bytes, cudaStream_t stream, bool early,
+cudaError_t launch_chained(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem_bytes, cudaStream_t stream,
                            const Args&... args) {
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -161,7 +161,7 @@ cudaError_t launch_chained(void (*kernel)(Params...), dim3 grid, dim3 block, siz
   config.dynamicSmemBytes = smem_bytes;
   config.stream = stream;
   config.attrs = &attr;
-  config.numAttrs = early ? 1 : 0;
+  config.numAttrs = 1;
   return cudaLaunchKernelEx(&config, kernel, args...);
 }
 
