@@ -16,7 +16,7 @@
 // accumulator is rescaled when it or R moves.  The warps' results merge in shared memory, the parts of a split row in
 // combine_few_kernel.
 //
-// One query over 4 rows x 12 heads x 32760 keys (405 MB): 70 us, 5.8 TB/s; over one such row 26 us, of which about 10 are
+// One query over 4 rows x 12 heads x 32760 keys (405 MB): 70 us, 5.8 TB/s; over one such row 25 us, of which about 10 are
 // launch, first tiles and merging.  With the queries as the products' 16 rows: 77 and 33 us.  9 to 16 queries: 85 and 33 us.
 #include <cuda.h>
 #include <cuda_bf16.h>
