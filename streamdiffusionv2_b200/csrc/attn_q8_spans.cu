@@ -262,7 +262,7 @@ attn_x_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
     tmem_alloc(smem_u32(const_cast<int*>(words + kWordTmem)), Sh::kTmemCols);
     tmem_relinquish();
   }
-  begin_after_previous_kernel();
+  wait_for_previous_kernel();
   if (threadIdx.x == 0) {
     for (int s = 0; s < n_stage; ++s) {  // the queries are wanted whatever the keys; the issuing thread waits for them
       mbar_expect_tx(bar(kBarQFull + s), kTileBytes);
@@ -288,6 +288,7 @@ attn_x_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  let_next_kernel_in();
   if (kSpans) {
     const bool some = span_hi > span_lo;
     const int lo = __reduce_min_sync(0xffffffffu, some ? span_lo : 0x7FFFFFFF);

@@ -66,17 +66,22 @@ enum WaitSite : int {
   BAD_STEP_PARAMS = 10  // not a wait: device-resident slot parameters were out of range, nothing written
 };
 
+// For kernels launched while the one before them still runs (launch_chained).  Everything in front of
+// wait_for_previous_kernel() is set-up that touches no global memory.  let_next_kernel_in() comes behind it, since the
+// kernel after this one takes it for granted that what came before this one has completed, and behind a block barrier that
+// follows the block's allocation of tensor memory: the next kernel's set-up may allocate too, waits for this kernel
+// with the columns in hand, and an allocation has no time limit.
+__device__ __forceinline__ void wait_for_previous_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_next_kernel_in() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+// Both, for kernels without tensor memory.
+__device__ __forceinline__ void begin_after_previous_kernel() {
+  wait_for_previous_kernel();
+  let_next_kernel_in();
+}
+
 // Spin on an mbarrier phase with a cycle budget.  `abort_flag` lives in shared memory and is
 // raised by whichever thread runs out first so that every other role leaves its loop promptly;
 // `status` (global) records the site.  Returns false when the wait was abandoned.
-// For kernels launched while the one before them still runs (launch_chained): everything in front of this call is set-up
-// that touches no global memory.  The kernel after this one may be set up from here on, not earlier: it takes it for
-// granted that what came before this kernel has completed.
-__device__ __forceinline__ void begin_after_previous_kernel() {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-}
-
 constexpr long long kWaitBudgetCycles = 1500000000LL;  // well under a second of SM clock
 
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag,

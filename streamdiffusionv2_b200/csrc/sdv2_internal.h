@@ -148,7 +148,7 @@ __device__ __forceinline__ uint32_t rms_scale_pair(uint32_t x, float rstd, uint3
 #endif
 
 // Launch `kernel` so that its set-up overlaps the end of the kernel before it on the stream, whoever's that is; every
-// thread of it calls begin_after_previous_kernel() before it touches global memory.
+// thread of it calls wait_for_previous_kernel() or begin_after_previous_kernel() before it touches global memory.
 template <typename... Params, typename... Args>
 cudaError_t launch_chained(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem_bytes, cudaStream_t stream,
                            const Args&... args) {
