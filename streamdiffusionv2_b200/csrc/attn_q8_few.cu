@@ -136,7 +136,7 @@ attn_few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       uint4 v = make_uint4(0u, 0u, 0u, 0u);
-      if (row < p.q_tokens) v = __ldg(reinterpret_cast<const uint4*>(qp + (i >> 1) * 64 + (i & 1) * 8));
+      if (row < p.q_tokens) v = *reinterpret_cast<const uint4*>(qp + (i >> 1) * 64 + (i & 1) * 8);
       qb[nb][2 * i][0] = v.x;
       qb[nb][2 * i][1] = v.y;
       qb[nb][2 * i + 1][0] = v.z;

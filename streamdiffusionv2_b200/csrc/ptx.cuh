@@ -71,6 +71,8 @@ enum WaitSite : int {
 // kernel after this one takes it for granted that what came before this one has completed, and behind a block barrier that
 // follows the block's allocation of tensor memory: the next kernel's set-up may allocate too, waits for this kernel
 // with the columns in hand, and an allocation has no time limit.
+// Such a kernel reads global memory with plain loads: ld.global.nc (__ldg) is for data that nobody writes while the kernel
+// runs, and this one's run begins while the kernel before it may still be writing its operands.
 __device__ __forceinline__ void wait_for_previous_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void let_next_kernel_in() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 // Both, for kernels without tensor memory.
@@ -79,11 +81,11 @@ __device__ __forceinline__ void begin_after_previous_kernel() {
   let_next_kernel_in();
 }
 
+constexpr long long kWaitBudgetCycles = 1500000000LL;  // well under a second of SM clock
+
 // Spin on an mbarrier phase with a cycle budget.  `abort_flag` lives in shared memory and is
 // raised by whichever thread runs out first so that every other role leaves its loop promptly;
 // `status` (global) records the site.  Returns false when the wait was abandoned.
-constexpr long long kWaitBudgetCycles = 1500000000LL;  // well under a second of SM clock
-
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag,
                                           int* status, int site, long long budget = kWaitBudgetCycles) {
   if (mbar_try_wait(bar, parity)) return true;

@@ -29,7 +29,7 @@ struct Raw8;
 template <>
 struct Raw8<__nv_bfloat16> {
   uint4 a;
-  __device__ __forceinline__ void load(const __nv_bfloat16* p) { a = __ldg(reinterpret_cast<const uint4*>(p)); }
+  __device__ __forceinline__ void load(const __nv_bfloat16* p) { a = *reinterpret_cast<const uint4*>(p); }
   __device__ __forceinline__ void get(float (&x)[8]) const {
     const uint32_t w[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
@@ -43,8 +43,8 @@ template <>
 struct Raw8<float> {
   uint4 a, b;
   __device__ __forceinline__ void load(const float* p) {
-    a = __ldg(reinterpret_cast<const uint4*>(p));
-    b = __ldg(reinterpret_cast<const uint4*>(p) + 1);
+    a = reinterpret_cast<const uint4*>(p)[0];
+    b = reinterpret_cast<const uint4*>(p)[1];
   }
   __device__ __forceinline__ void get(float (&x)[8]) const {
     const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
@@ -164,7 +164,7 @@ rope_kv_append_q8_kernel(const __grid_constant__ Q8AppendParams qp) {
   rv.load(v_src);
   double2 cs[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) cs[i] = table_entry(p, c * 4 + i, row_start_frame(p, b) + f, y, x);
+  for (int i = 0; i < 4; ++i) cs[i] = *table_place(p, c * 4 + i, row_start_frame(p, b) + f, y, x);
   T* q_dst = static_cast<T*>(p.q_out.ptr) + b * p.q_out.stride_row + t * p.q_out.stride_tok + h_first * p.q_out.stride_head + c * 8;
   uint8_t* k_dst = static_cast<uint8_t*>(p.k_cache.ptr) + b * p.k_cache.stride_row + slot * p.k_cache.stride_tok +
                    h_first * p.k_cache.stride_head + c * 8;
@@ -262,9 +262,9 @@ __global__ void __launch_bounds__(256) kv_read_q8_kernel(const __grid_constant__
         const sdv2_view& cv = which ? p.v : p.k;
         const sdv2_view& ev = which ? p.v_exp : p.k_exp;
         const sdv2_view& ov = which ? p.v_out : p.k_out;
-        raw[u][which] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(cv.ptr) + b * cv.stride_row +
-                                                             src * cv.stride_tok + h * cv.stride_head + c));
-        e[u][which] = __ldg(static_cast<const signed char*>(ev.ptr) + b * ev.stride_row + src * ev.stride_tok + h * ev.stride_head);
+        raw[u][which] = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(cv.ptr) + b * cv.stride_row +
+                                                        src * cv.stride_tok + h * cv.stride_head + c);
+        e[u][which] = static_cast<const signed char*>(ev.ptr)[b * ev.stride_row + src * ev.stride_tok + h * ev.stride_head];
         out[u][which] = b * ov.stride_row + dst * ov.stride_tok + h * ov.stride_head + c;
       }
     }

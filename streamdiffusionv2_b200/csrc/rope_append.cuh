@@ -19,9 +19,13 @@ __device__ __forceinline__ void rope_pair(double a, double b, double2 cs, float&
 __device__ __forceinline__ int fast_div(uint32_t n, uint32_t m) { return static_cast<int>(m == 0 ? n : __umulhi(n, m)); }
 
 // table entry for complex column `col` of a token at (time row, grid row y, grid column x)
-__device__ __forceinline__ double2 table_entry(const AppendParams& p, int col, int64_t trow, int y, int x) {
+__device__ __forceinline__ const double2* table_place(const AppendParams& p, int col, int64_t trow, int y, int x) {
   const int64_t row = col < p.cols_t ? trow : (col < p.cols_t + p.cols_h ? y : x);
-  return __ldg(p.table + row * p.half + col);
+  return p.table + row * p.half + col;
+}
+// ... for kernels that start when everything before them has ended
+__device__ __forceinline__ double2 table_entry(const AppendParams& p, int col, int64_t trow, int y, int x) {
+  return __ldg(table_place(p, col, trow, y, x));
 }
 
 // Per-row slot parameters come from the launch parameters or, for launches that must not carry

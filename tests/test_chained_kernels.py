@@ -34,3 +34,11 @@ def test_tensor_memory_is_held_before_the_next_kernel_may_come_in(name):
         assert release >= begin.start() and body.count("let_next_kernel_in()") <= 1, kernel
         if "tmem_alloc(" in body:
             assert "__syncthreads()" in body[body.index("tmem_alloc("):release], kernel
+
+
+@pytest.mark.parametrize("name", SOURCES + ["q8.cuh", "attn_items.cuh"])
+def test_no_load_promises_that_nobody_writes_its_operands_meanwhile(name):
+    """ld.global.nc and __ldg hold for data that stays as it is for the kernel's whole run, which here begins while the
+    kernel in front may still be writing it; table_entry is the append's lookup that uses them."""
+    text = re.sub(r"//[^\n]*", "", open(os.path.join(CSRC, name)).read())
+    assert not re.search(r"__ldg|\.nc\b|table_entry\(", text), name
