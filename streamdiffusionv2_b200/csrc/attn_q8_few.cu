@@ -72,6 +72,7 @@ __device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 
 __device__ __forceinline__ int result_chunk(int query, int c4) { return c4 ^ ((query >> 1) & 3); }
 
 constexpr int kQueryExp = 110;   // queries enter the product as q * 2^kQueryExp
+constexpr int kMaxScaleExp = 127 - (133 - kQueryExp);  // largest K exponent whose factor of a score fp32 holds
 constexpr int kWeightExp = 120;  // weights enter the product as p * 2^(e - R + kWeightExp)
 
 // kN: eights of query rows
@@ -145,8 +146,9 @@ attn_few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
   }
   __syncthreads();  // the abort flag belongs to all warps
 
-  // scale the queries by 2^110, a row whose largest element would pass 2^120 by less (none, with an infinity or NaN: its
-  // scores are not finite either way)
+  // scale the queries by 2^110; a row whose largest element would pass 2^120 by less (none, with an infinity or NaN: its
+  // scores are not finite either way), one whose elements all lie below 2^-17 by 2^127: only keys near the largest that
+  // the format holds give it scores that matter, and at 2^110 such products would be subnormal numbers
   float row_fix[kN][2];  // of queries 2 t4, 2 t4 + 1, as all that follows
   bool plain = true;
 #pragma unroll
@@ -154,10 +156,11 @@ attn_few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
     uint32_t top = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) top = __vmaxu2(top, __vmaxu2(qb[nb][i][0] & 0x7FFF7FFFu, qb[nb][i][1] & 0x7FFF7FFFu));
-    top = max(top & 0xFFFFu, top >> 16) >> 7;  // exponent field
+    top = max(top & 0xFFFFu, top >> 16);
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    const int qs = min(max(246 - static_cast<int>(top), 0), kQueryExp);
+    const int field = static_cast<int>(top >> 7);  // the exponent's
+    const int qs = top != 0 && field < 127 - 17 ? 127 : min(max(246 - field, 0), kQueryExp);
     const uint32_t q2 = q8::scale_bits(qs, false);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -235,7 +238,7 @@ attn_few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
     // this lane's key: its exponents as factors of a score and of a weight, and R
     const int left = key1 - first;
     const int ref_new = max(ref_v, __reduce_max_sync(0xffffffffu, exp_v));
-    float fk = fmaxf(attnx::exp2_int(exp_k + 133 - kQueryExp) * p.scale_log2, 1.17549435e-38f);
+    float fk = fmaxf(attnx::exp2_int(min(exp_k, kMaxScaleExp) + 133 - kQueryExp) * p.scale_log2, 1.17549435e-38f);
     float fv = attnx::exp2_int(exp_v - ref_new + kWeightExp);
     if (exp_k == q8::kNotFinite) fk = NAN;
     if (exp_v == q8::kNotFinite) fv = NAN;
@@ -258,6 +261,20 @@ attn_few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
         for (int nb = 0; nb < kN; ++nb)
 #pragma unroll
           for (int i = 0; i < 4; ++i) s[kb][nb][i] *= row_fix[nb][i & 1];
+    }
+    if (__any_sync(0xffffffffu, exp_k > kMaxScaleExp)) {  // what fk could not take
+      const float rest = attnx::exp2_int(max(exp_k - kMaxScaleExp, 0));
+#pragma unroll
+      for (int kb = 0; kb < kBlocks; ++kb)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float f = __shfl_sync(0xffffffffu, rest, kb * 16 + i * 8 + g);
+#pragma unroll
+          for (int nb = 0; nb < kN; ++nb) {
+            s[kb][nb][2 * i] *= f;
+            s[kb][nb][2 * i + 1] *= f;
+          }
+        }
     }
     if (left < kKeys) {
 #pragma unroll
