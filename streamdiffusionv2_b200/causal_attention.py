@@ -123,7 +123,11 @@ def block_causal_spans(frames: int, frame_tokens: int, frames_per_block: int, de
                        window_frames: int = -1) -> KeySpans:
     """Spans of a clip processed in one pass: a token attends its own block of frames and every block before it
     (the training branch's mask, models/wan/causal_model.py:220-249), with window_frames > 0 only the last window_frames
-    frames up to its block's end."""
+    frames up to its block's end (the clip's end for a last block cut short).  A window shorter than a block, in which a
+    block's early frames would not attend themselves, is refused."""
+    if frames_per_block < 1 or 0 < window_frames < frames_per_block:
+        raise ValueError(f"blocks of {frames_per_block} frames with a window of {window_frames}: a block has at least one "
+                         "frame and the window at least a block")
     t = torch.arange(frames * frame_tokens, device=device)
     block = frames_per_block * frame_tokens
     end = ((t // block + 1) * block).clamp_max(frames * frame_tokens)

@@ -367,7 +367,8 @@ class CausalWanModel(nn.Module):
         num_frame_per_block) attends itself and what came before it (see `causal_attention.block_causal_spans`), as
         streaming it block by block through a cache that never evicts would.  x [B, C, F, H, W]; t [B, F] timesteps;
         context [B, Lt, text_dim]; `context_lens`, where given, the prompts' lengths: text tokens past them are not
-        attended.  bf16 on CUDA; inference only.  Returns [B, C, F, H, W]."""
+        attended; `window_frames` > 0 (at least a block): only the last window_frames frames up to a block's end.  bf16 on CUDA;
+        inference only.  Returns [B, C, F, H, W]."""
         device = self.patch_embedding.weight.device
         if self.freqs.device != device:
             self.freqs = self.freqs.to(device)
