@@ -357,7 +357,7 @@ size_t sdv2_attn_q8_scratch_bytes(int rows, int q_tokens, int heads, int64_t cac
  * Covers WanT2VCrossAttention.forward with context_lens (models/wan/wan_base/modules/model.py:161-194) and the masks of
  * CausalWanSelfAttention.forward without a cache (models/wan/causal_model.py:220-249).
  *
- * bf16 in and out, fp32 accumulate, head_dim 128; k / v stride_row may be 0.  begin_dev (NULL: 0) and end_dev: device
+ * bf16 in and out, fp32 accumulate, head_dim 128; stride_row of k and of v may be 0, of both or neither.  begin_dev (NULL: 0) and end_dev: device
  * int32, element strides per row and per query, 0 allowed (one span for all); read when the kernel runs.
  * K and V of keys that no query attends may hold anything, NaN included.
  * scratch_dev, status_dev: as for sdv2_attn_kvcache_q8, with sdv2_attn_spans_scratch_bytes().

@@ -363,6 +363,7 @@ PyObject* spans(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int64_t kv[4] = {rows, k.size(1), heads, dim}, sp[2] = {rows, tokens};
     const at::IntArrayRef s4(kv, 4), s2(sp, 2);
     const sdv2_view vk = view4(k, s4, at::kBFloat16, dev, what, "k"), vv = view4(tensor(a[2], what, "v"), s4, at::kBFloat16, dev, what, "v");
+    if ((vk.stride_row == 0) != (vv.stride_row == 0)) refuse("attn_spans: k and v are broadcast over rows both or neither");
     const at::Tensor& end = tensor(a[4], what, "end");
     expect(end, s2, at::kInt, dev, what, "end");
     at::Tensor begin;

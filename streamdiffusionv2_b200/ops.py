@@ -370,8 +370,8 @@ def attn_kvcache_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
 def attn_spans(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, begin: Optional[torch.Tensor], end: torch.Tensor, *,
                out: Optional[torch.Tensor] = None, softmax_scale: Optional[float] = None) -> torch.Tensor:
     """Attention in which query i of row b attends the keys begin[b, i] <= j < end[b, i] only: prompt lengths,
-    block-causal clips, clips packed into one row, windows.  q [B, N, H, 128], k / v [B, S, H, 128] bf16 (k / v may be
-    stride-0 expands over rows); begin (None: 0) and end int32 [B, N] on the device, any strides (an expanded [B, 1]
+    block-causal clips, clips packed into one row, windows.  q [B, N, H, 128], k / v [B, S, H, 128] bf16 (both
+    or neither may be stride-0 expands over rows); begin (None: 0) and end int32 [B, N] on the device, any strides (an expanded [B, 1]
     does for one span per row).  Spans are clipped to the keys there are; a query with an empty span gets 0.  K and V of
     keys that no query attends may hold anything.  No gradient is recorded."""
     args = (q, k, v, begin, end, out, softmax_scale, _status_ptr(q))
