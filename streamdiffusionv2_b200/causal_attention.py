@@ -135,11 +135,15 @@ def block_causal_spans(frames: int, frame_tokens: int, frames_per_block: int, de
     return KeySpans(begin, end.int().expand(rows, -1))
 
 
+def _refuse_gradients(what: str, *tensors) -> None:
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise RuntimeError(f"{what} records no gradient: call it under torch.no_grad()")
+
+
 def clip_attention(q, k, v, grid_sizes, freqs, spans: KeySpans, norm=None):
     """Rope and attention of a whole clip without a cache: already projected q/k/v [B, N, H, D] in bf16, `norm` as for
     `cached_attention`.  Inference only (no gradient is recorded)."""
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v)):
-        raise RuntimeError("attention over key spans records no gradient: call it under torch.no_grad()")
+    _refuse_gradients("attention over key spans", q, k, v)
     B, n, H, D = q.shape
     grid = tuple(int(x) for x in grid_sizes[0].tolist())
     table = ops.rope_table_device(freqs, q.device)
@@ -159,6 +163,8 @@ def cached_attention(attn_module, q, k, v, grid_sizes, freqs, kv_cache, current_
     q8 = "k_exp" in kv_cache
     if q8 and q.dtype != torch.bfloat16:     # before the cache is written
         raise ValueError(f"attention over an 8-bit cache takes bf16 tensors, not {q.dtype}")
+    if q8:
+        _refuse_gradients("attention over an 8-bit cache", q, k, v)
     f, gh, gw = (int(x) for x in grid_sizes[0].tolist())
     frame_tokens = gh * gw
     starts = host_starts(current_start, B)
@@ -324,12 +330,15 @@ def cross_attention_forward(self, x, context, context_lens, crossattn_cache=None
     first call after `is_init` was cleared and read from the cache afterwards.  `context_lens` (one per row: a tensor
     or ints), where given, keeps a row's queries to its first context_lens tokens; a row of length 0 gets 0."""
     b, n, d = x.size(0), self.num_heads, self.head_dim
-    q = _qk_norm(self.norm_q, self.q(x)).view(b, -1, n, d)
+    q = self.q(x)
+    want = [q]           # before the norms, which keep no gradient
+    q = _qk_norm(self.norm_q, q).view(b, -1, n, d)
     if crossattn_cache is not None:
         if not crossattn_cache["is_init"]:
             crossattn_cache["is_init"] = True
-            k = _qk_norm(self.norm_k, self.k(context)).view(b, -1, n, d)
-            v = self.v(context).view(b, -1, n, d)
+            k, v = self.k(context), self.v(context).view(b, -1, n, d)
+            want.append(k)
+            k = _qk_norm(self.norm_k, k).view(b, -1, n, d)
             crossattn_cache["k"] = k
             crossattn_cache["v"] = v
         else:
@@ -341,8 +350,7 @@ def cross_attention_forward(self, x, context, context_lens, crossattn_cache=None
     if context_lens is not None:
         if q.dtype != torch.bfloat16:
             raise NotImplementedError("per-sample context lengths need bf16 tensors")
-        if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v)):
-            raise RuntimeError("attention with context lengths records no gradient: call it under torch.no_grad()")
+        _refuse_gradients("attention with context lengths", *want, q, k, v)
         lens = torch.as_tensor(context_lens, dtype=torch.int32, device=q.device).reshape(b, 1)
         out = ops.attn_spans(q, k, v, None, lens.expand(b, q.shape[1]))
     elif q.dtype == torch.bfloat16:

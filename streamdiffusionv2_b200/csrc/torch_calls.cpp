@@ -7,6 +7,7 @@
 // whose addresses bind() was given do the rest.
 #include <Python.h>
 #include <ATen/ATen.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
@@ -127,6 +128,15 @@ void on_cuda(const at::Device& d, const char* what) {
   if (!d.is_cuda()) refuse(std::string(what) + ": expected CUDA tensors (there is no CPU path)");
 }
 
+// Nothing here records a gradient: while gradients are recorded a tensor that wants one is refused, outputs too.
+template <typename... Tensors>
+void no_gradient(const char* what, const Tensors&... t) {
+  if (c10::GradMode::is_enabled() && (t.requires_grad() || ...)) {
+    PyErr_SetString(PyExc_RuntimeError, (std::string(what) + " records no gradient: call it under torch.no_grad()").c_str());
+    throw Refused();
+  }
+}
+
 float scale_of(PyObject* o, int64_t head_dim) {
   if (o == Py_None) return static_cast<float>(1.0 / std::sqrt(static_cast<double>(head_dim)));
   const double x = PyFloat_AsDouble(o);
@@ -209,7 +219,9 @@ PyObject* append_q8(PyObject*, PyObject* const* a, Py_ssize_t n) {
     Py_DECREF(grid);
     if (PyErr_Occurred()) throw Refused();
     if (!three) refuse("rope_kv_append_q8: grid must be (frames, height, width)");
+    no_gradient(what, q, tensor(a[1], what, "k"), tensor(a[2], what, "v"));
     const at::Tensor out = a[11] != Py_None ? tensor(a[11], what, "q_out") : (on_cuda(dev, what), at::empty(q.sizes(), q.options()));
+    no_gradient(what, out);
     const sdv2_view vq = view4(q, q.sizes(), type, dev, what, "q"), vk = view4(tensor(a[1], what, "k"), q.sizes(), type, dev, what, "k"),
                     vv = view4(tensor(a[2], what, "v"), q.sizes(), type, dev, what, "v"),
                     vo = view4(out, q.sizes(), type, dev, what, "q_out");
@@ -288,7 +300,6 @@ PyObject* read_q8(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int dtype = code_of(type, what);
     const int64_t shape[4] = {rows, tokens, heads, 128};
     const at::IntArrayRef s4(shape, 4);
-    on_cuda(dev, what);
     const Ints<int64_t> begin(a[4], rows, what);
     at::Tensor out[2];
     if (a[7] != Py_None) {
@@ -299,7 +310,10 @@ PyObject* read_q8(PyObject*, PyObject* const* a, Py_ssize_t n) {
       for (int i = 0; two && i < 2; ++i) out[i] = THPVariable_Unpack(PySequence_Fast_GET_ITEM(pair, i));
       Py_DECREF(pair);
       if (!two) refuse("kv_read_q8: out must be two tensors");
+      no_gradient(what, out[0], out[1]);
+      on_cuda(dev, what);
     } else {
+      on_cuda(dev, what);
       for (auto& t : out) t = at::empty(s4, at::TensorOptions().dtype(type).device(dev));
     }
     const sdv2_view ko = view4(out[0], s4, type, dev, what, "out[0]"), vo = view4(out[1], s4, type, dev, what, "out[1]");
@@ -331,8 +345,11 @@ PyObject* attn_q8(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (q.scalar_type() != at::kBFloat16) refuse("attn_kvcache_q8: the tensor-core attention kernel takes bf16");
     const Cache c = cache_of(a + 1, dev, rows, heads, dim, what);
     const Ints<int32_t> lens(a[5], rows, what);
-    on_cuda(dev, what);
+    no_gradient(what, q);
+    if (a[6] == Py_None) on_cuda(dev, what);
     const at::Tensor out = out_like(q, a[6], what);
+    no_gradient(what, out);
+    on_cuda(dev, what);
     const sdv2_view vq = view4(q, q.sizes(), at::kBFloat16, dev, what, "q"), vo = view4(out, q.sizes(), at::kBFloat16, dev, what, "out");
     const float scale = scale_of(a[7], dim);
     void* status = PyLong_AsVoidPtr(a[8]);
@@ -371,8 +388,11 @@ PyObject* spans(PyObject*, PyObject* const* a, Py_ssize_t n) {
       begin = tensor(a[3], what, "begin");
       expect(begin, s2, at::kInt, dev, what, "begin");
     }
-    on_cuda(dev, what);
+    no_gradient(what, q, k, tensor(a[2], what, "v"));
+    if (a[5] == Py_None) on_cuda(dev, what);
     const at::Tensor out = out_like(q, a[5], what);
+    no_gradient(what, out);
+    on_cuda(dev, what);
     const sdv2_view vq = view4(q, q.sizes(), at::kBFloat16, dev, what, "q"), vo = view4(out, q.sizes(), at::kBFloat16, dev, what, "out");
     const float scale = scale_of(a[6], dim);
     void* status = PyLong_AsVoidPtr(a[7]);

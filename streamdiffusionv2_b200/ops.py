@@ -332,7 +332,8 @@ def rope_kv_append_q8(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache
     [dst_begin[b], dst_begin[b] + N), one power-of-two exponent per (token, head): e = max(floor(log2(max|x|)) - 6, -126),
     magnitudes min(rint(|x| / 2^e), 127).  A head vector with a value that is not finite reads back as NaN.
     q, k, v [B, N, H, 128] bf16 or fp32; `index_tensors`, `index_values`, `step_params` as for `rope_kv_append`.
-    Returns the roped q, the same bits as `rope_kv_append`'s."""
+    Returns the roped q, the same bits as `rope_kv_append`'s.  No gradient is recorded: tensors that
+    want one are refused while gradients are on, here and in the calls below."""
     args = (q, k, v, k_cache, v_cache, k_exp, v_exp, table, grid, start_frames, dst_begin, q_out, index_tensors, index_values,
             step_params, _status_ptr(q))
     if _log is None:
