@@ -345,7 +345,9 @@ def cross_attention_forward(self, x, context, context_lens, crossattn_cache=None
             k = crossattn_cache["k"]
             v = crossattn_cache["v"]
     else:
-        k = self.norm_k(self.k(context)).view(b, -1, n, d)
+        k = self.k(context)
+        want.append(k)
+        k = self.norm_k(k).view(b, -1, n, d)
         v = self.v(context).view(b, -1, n, d)
     if context_lens is not None:
         if q.dtype != torch.bfloat16:
