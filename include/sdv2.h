@@ -328,7 +328,8 @@ int sdv2_residual_layernorm(const void* x, const void* y, const void* gate, int6
  *   (`dtype`; both exact).  begin: host int64[rows], begin[b] + tokens <= cache_tokens.  Cache rows may be broadcast
  *   (stride_row 0), here and in the attention.  heads <= 8191, there too.
  * sdv2_attn_kvcache_q8: sdv2_attn_kvcache over the values the cache holds.  seq_lens[b] may be 0: that row's output is
- *   0.  Cache bytes and exponents at and beyond seq_lens[b] may hold anything.  Scores (q . k, scaled) have to stay
+ *   0.  Cache bytes and exponents at and beyond seq_lens[b] may hold anything.  V counts to within 2^-120 of the largest
+ *   of its row and head (exponents further apart than that are not kept apart).  Scores (q . k, scaled) have to stay
  *   within fp32's range.  scratch_dev: at least sdv2_attn_q8_scratch_bytes() bytes (may be 0: then NULL), 32-byte
  *   aligned, no initialisation needed; one call's own, calls that may overlap on the GPU need one each.  status_dev as for
  *   sdv2_rope_kv_append.
@@ -357,9 +358,11 @@ size_t sdv2_attn_q8_scratch_bytes(int rows, int q_tokens, int heads, int64_t cac
  * Covers WanT2VCrossAttention.forward with context_lens (models/wan/wan_base/modules/model.py:161-194) and the masks of
  * CausalWanSelfAttention.forward without a cache (models/wan/causal_model.py:220-249).
  *
- * bf16 in and out, fp32 accumulate, head_dim 128; stride_row of k and of v may be 0, of both or neither.  begin_dev (NULL: 0) and end_dev: device
- * int32, element strides per row and per query, 0 allowed (one span for all); read when the kernel runs.
- * K and V of keys that no query attends may hold anything, NaN included.
+ * bf16 in and out, fp32 accumulate, head_dim 128; stride_row of k and of v may be 0, of both or neither.  begin_dev (NULL:
+ * 0) and end_dev: device int32, element strides per row and per query, 0 allowed (one span for all); read when the kernel
+ * runs.  K and V of keys that no query of a row attends may hold anything, NaN included.  An infinity or NaN in a V that
+ * some query attends may reach the queries of the same row and head around that query (up to 255 to either side) whose own
+ * span leaves it out: clips packed into one row are not kept apart there, rows are.  K is.
  * scratch_dev, status_dev: as for sdv2_attn_kvcache_q8, with sdv2_attn_spans_scratch_bytes().
  */
 int sdv2_attn_spans(const sdv2_view* q, const sdv2_view* k, const sdv2_view* v, const sdv2_view* out, int rows,

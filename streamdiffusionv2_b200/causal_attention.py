@@ -328,7 +328,8 @@ def self_attention_forward(self, x, seq_lens, grid_sizes, freqs, block_mask, kv_
 def cross_attention_forward(self, x, context, context_lens, crossattn_cache=None):
     """Drop-in for WanT2VCrossAttention.forward: K/V of the text context are computed on the
     first call after `is_init` was cleared and read from the cache afterwards.  `context_lens` (one per row: a tensor
-    or ints), where given, keeps a row's queries to its first context_lens tokens; a row of length 0 gets 0."""
+    or ints), where given, keeps a row's queries to its first context_lens tokens; a row of length 0 gets 0.  A device
+    int32 tensor is used as it is; anything else is copied to the device by every call, which cannot be recorded into a graph."""
     b, n, d = x.size(0), self.num_heads, self.head_dim
     q = self.q(x)
     want = [q]           # before the norms, which keep no gradient

@@ -602,14 +602,18 @@ static void set_partials(sdv2::AttnXParams& p, void* scratch, int slots) {
 // query tiles and takes shared-memory bandwidth from the tensor cores (about 4400 cycles a key tile against 3250);
 // expanding them to bf16 scratch first costs 6 bytes of HBM traffic a value once, 3900 cycles' share of a key tile.  So
 // from four pairs of query tiles on (more than 768 queries) the cache is expanded first, a group of heads at a time so
-// that the scratch stays near 1 GiB: 600 queries over 32760 keys x 12 heads take 165 us expanding in the kernel and 183
-// expanding first, 800 queries 216 and 221, over 2 rows x 9000 keys x 40 heads 411 and 396.
+// that the scratch stays near 1 GiB.  Microseconds expanding in the kernel / first, at 768, 1000, 1200 and 1500 queries:
+// 5 heads x 9000 keys 33 / 33, 41 / 39.5, 50 / 46, 56 / 51; 12 heads x 4680 39 / 39, 48 / 46, 62 / 57, 64 / 59; 12 x 32760
+// 180 / 207, 235 / 254, 314 / 319, 343 / 343; 2 rows x 40 heads x 9000 353 / 394, 427 / 457, 538 / 550, 632 / 629.  So the
+// switch could lie two pairs later where tiles fill the GPU several times over; the rule takes the one place that serves
+// small calls too.
 //
 // Up to kFewQueries queries have a kernel of their own that never leaves the cache's bytes for shared-memory tiles: at
-// 32760 keys x 12 heads 50 us for 32 queries (two blocks' worth) against 61 here for 33, at four such rows 160 against 187.
+// 32760 keys x 12 heads (100 MB, in the L2 from call to call) 46 us for 32 queries (two blocks' worth, each walking the
+// cache: 30 us for 16) against 57 here for 33, at four such rows 158 against 184.
 //
-// A part of a split tile has at least kMinPart tiles of 128 keys: with two, 200 queries over 4000 keys x 2 heads take 19 us,
-// with four 23, with eight 31; one token over them 12 us, 13.5 and 17.
+// A part of a split tile has at least kMinPart tiles of 128 keys: with two, 200 queries over 4000 keys x 2 heads take 15.5
+// us, with four 18.8, with eight 25.7; one token over them 8.4 us, 8.1 and 10.9.
 constexpr int kFewQueries = 32, kMinPart = 2;
 constexpr int kSetup = 2, kFewSetup = 4;  // set-up, first loads and epilogue in key tiles' time (6000 to 3800 cycles; 15000 to 4200)
 struct Q8Run {

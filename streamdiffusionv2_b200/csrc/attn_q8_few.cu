@@ -332,6 +332,7 @@ attn_few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
             w[q] = ex2_approx(s[kb][nb][2 * i + q] - (m[nb][q] == -INFINITY ? 0.f : m[nb][q]));
             l[nb][q] += w[q];
           }
+          // bf16 as in the tensor-core kernels: 2^-9 of the output, as much as its own rounding
           pb[kb][nb][i] = transpose8(pack_bf16x2(w[0] * f, w[1] * f));  // now of query g, keys 2 t4, 2 t4 + 1
         }
       }

@@ -13,14 +13,17 @@
 //
 // Spans.  Row i attends keys [begin_i, end_i).  A CTA walks the key tiles between the smallest begin and the largest
 //   end of its rows; a thread masks its own row, and only in tiles that its span does not cover.  V rows that no row
-//   of the CTA attends are cleared on chip (0 x NaN would reach the output otherwise).  Rows with an empty span give 0.
+//   of the CTA attends are cleared on chip (0 x NaN would reach the output otherwise); one that some row of it attends stays,
+//   so an infinity or NaN in it reaches the CTA's other rows too.  Rows with an empty span give 0.
 //
 // Split tiles write unnormalised O, the running maximum, sum and V exponent to scratch; combine_kernel merges them.
 //
 // Bound by the chain S -> softmax -> P V of a query tile, two of which share the tensor pipe and the exp unit (both some
 // 60 % busy): 3800 cycles a step of 128 keys for 256 queries.  14040 queries in three blocks over 14040 keys x 12 heads:
-// 664-676 us, 1.2 PFLOP/s (782 us in long runs under the power cap); 2 x 3120 queries over 32760 expanded keys x 12 heads 1.0
-// ms of 1.1; expanded here, 256 queries over 32760 keys x 12 heads 71 us.
+// 664-676 us, 1.2 PFLOP/s, where the clock stays up (756-786 us elsewhere and in long runs under the power cap); 2 x 3120
+// queries over 32760 keys x 12 heads expanded first 1.15 ms of 1.24 in such a run, 2 % more than the bf16 cache kernel takes
+// over the same scratch (it refuses empty rows and keeps its partial results in the one workspace of a device, where a call
+// here has its own); expanded here, 256 queries over 32760 keys x 12 heads 73 us.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -648,6 +651,8 @@ attn_x_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
           }
         }
         const float m_sub = m_used == -INFINITY ? 0.f : m_used;  // no key yet: exponentials of -inf, not of -inf + inf
+        // P goes to bf16 because the product takes nothing wider beside V's bf16; the sum keeps fp32.  It puts the output off
+        // by 2^-9 of itself (root mean square, values of random signs), as much as rounding the output to bf16 does.
         float sum0 = 0.f, sum1 = 0.f;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
@@ -870,12 +875,16 @@ cudaError_t launch_attn_spans(const CUtensorMap& tm_q, const CUtensorMap& tm_k, 
 // share is empty costs little.  Tiles before the tail run late queries first.
 //
 // One query tile to a CTA up to kShortKeys keys, two beyond (3120 queries, microseconds with one and with two): 300 keys
-// x 12 heads 23.2 and 25.2, 512 x 48 heads 60.5 and 65, 1024 x 24 heads 57.8 and 60.2; 2048 x 24 heads 91.6 and 89.2, 4680 x
-// 12 heads 155 and 148.  That holds for 128 queries too, whose second tile is empty: its ring is deeper (12 heads x
-// 16384 keys 66 and 48).  A part has at least two key tiles where
-// everything fits one wave (1001 tokens x 3 heads: 20.5 us against 22.5 with four; 256 queries over 1536 keys 22.5 against
-// 24.6; both 18.4 with today's merging), else four: the tail then overlaps the waves before it, and merging two parts of two tiles each costs more than
-// it saves (the 512 keys above: 43.4 against 47.5 us).
+// x 12 heads 21.2 and 22.1, 512 x 48 heads 58.5 and 60.7, 1024 x 24 heads 53.7 and 54.9; 2048 x 24 heads 94.0 and 89.2, 4680 x
+// 12 heads 107 and 99.5.  That holds for 128 queries too, whose second tile is empty: its ring is deeper (12 heads x
+// 16384 keys 34.4 and 30.0).
+//
+// A part has at least two key tiles where everything fits one wave, else four.  One wave, with two and with four: 1001 tokens
+// in five clips x 3 heads 10.9 and 12.3 us, 2 x 200 queries over 700 keys x 6 heads 12.4 and 15.5, 256 over 1536 x 12 heads 16.1
+// and 16.9 (against it 600 over 800 x 12 heads, 21.0 and 18.0).  Beyond, the tail overlaps the waves before it, and merging
+// parts of two tiles each mostly costs more than it saves: 4 x 3120 queries over text of 512, 77, 226 and 0 keys x 12 heads
+// 42.7 and 40.0, 3120 over 512 x 48 heads 60.7 and 59.0, over 2048 x 24 heads 88.6 and 87.9 (against it 1024 x 13 heads, 34.0
+// and 36.3).
 int plan_spans(AttnXParams& p, int sms) {
   constexpr int kShortKeys = 1024;
   p.tiles = p.kv_tokens <= kShortKeys ? 1 : 2;

@@ -358,9 +358,9 @@ def attn_kvcache_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
                     v_exp: torch.Tensor, seq_lens: Sequence[int], *, out: Optional[torch.Tensor] = None,
                     softmax_scale: Optional[float] = None) -> torch.Tensor:
     """`attn_kvcache` over an 8-bit cache: softmax(q k^T scale) v over the values that cache[b, :seq_lens[b]] holds
-    (bf16 q and output).  seq_lens[b] may be 0: that row's output is 0.  Cache rows may be broadcast.  Scratch comes from
-    PyTorch's allocator; above 768 queries it holds bf16 K and V of a group of heads, about 1 GiB at most (one head at
-    least).  No gradient is recorded."""
+    (bf16 q and output).  seq_lens[b] may be 0: that row's output is 0.  Cache rows may be broadcast.  Scores have to stay
+    within fp32's range.  Scratch comes from PyTorch's allocator; above 768 queries it holds bf16 K and V of a group of
+    heads, about 1 GiB at most (one head at least).  No gradient is recorded."""
     args = (q, k_cache, v_cache, k_exp, v_exp, seq_lens, out, softmax_scale, _status_ptr(q))
     if _log is None:
         return N.calls().attn_q8(*args)
@@ -374,7 +374,9 @@ def attn_spans(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, begin: Optiona
     block-causal clips, clips packed into one row, windows.  q [B, N, H, 128], k / v [B, S, H, 128] bf16 (both
     or neither may be stride-0 expands over rows); begin (None: 0) and end int32 [B, N] on the device, any strides (an expanded [B, 1]
     does for one span per row).  Spans are clipped to the keys there are; a query with an empty span gets 0.  K and V of
-    keys that no query attends may hold anything.  No gradient is recorded."""
+    keys that no query of a row attends may hold anything; an infinity or NaN in a V that some query attends may reach
+    the queries around that one (up to 255 to either side) whose own span leaves it out, so clips packed into one row
+    are not kept apart there.  No gradient is recorded."""
     args = (q, k, v, begin, end, out, softmax_scale, _status_ptr(q))
     if _log is None:
         return N.calls().spans(*args)
