@@ -329,10 +329,10 @@ int sdv2_residual_layernorm(const void* x, const void* y, const void* gate, int6
  *   (stride_row 0), here and in the attention.  heads <= 8191, there too.
  * sdv2_attn_kvcache_q8: sdv2_attn_kvcache over the values the cache holds.  seq_lens[b] may be 0: that row's output is
  *   0.  Cache bytes and exponents at and beyond seq_lens[b] may hold anything.  V counts to within 2^-120 of the largest
- *   of its row and head (exponents further apart than that are not kept apart).  Scores (q . k, scaled) have to stay
- *   within fp32's range.  scratch_dev: at least sdv2_attn_q8_scratch_bytes() bytes (may be 0: then NULL), 32-byte
- *   aligned, no initialisation needed; one call's own, calls that may overlap on the GPU need one each.  status_dev as for
- *   sdv2_rope_kv_append.
+ *   of its row and head (exponents further apart than that are not kept apart).  Scores (q . k, scaled) and softmax_scale
+ *   times the largest K have to stay within fp32's range.  scratch_dev: at least sdv2_attn_q8_scratch_bytes() bytes (may
+ *   be 0: then NULL), 32-byte aligned, no initialisation needed; one call's own, calls that may overlap on the GPU need one
+ *   each.  status_dev as for sdv2_rope_kv_append.
  */
 int sdv2_rope_kv_append_q8(const sdv2_view* q, const sdv2_view* k, const sdv2_view* v, const sdv2_view* q_out,
                            const sdv2_view* k_cache, const sdv2_view* v_cache, const sdv2_view* k_exp,

@@ -16,8 +16,8 @@
 // accumulator is rescaled when it or R moves.  The warps' results merge in shared memory, the parts of a split row in
 // combine_few_kernel.
 //
-// One query over 4 rows x 12 heads x 32760 keys (405 MB): 70 us, 5.8 TB/s; over one such row 25 us, of which about 10 are
-// launch, first tiles and merging.  With the queries as the products' 16 rows: 77 and 33 us.  9 to 16 queries: 85 and 33 us.
+// One query over 4 rows x 12 heads x 32760 keys (405 MB): 70-71 us, 5.7 TB/s; over one such row 25 us, of which about 10 are
+// launch, first tiles and merging.  With the queries as the products' 16 rows: 77 and 33 us.  9 to 16 queries: 85-91 and 33 us.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -72,7 +72,8 @@ __device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 
 __device__ __forceinline__ int result_chunk(int query, int c4) { return c4 ^ ((query >> 1) & 3); }
 
 constexpr int kQueryExp = 110;   // queries enter the product as q * 2^kQueryExp
-constexpr int kMaxScaleExp = 127 - (133 - kQueryExp);  // largest K exponent whose factor of a score fp32 holds
+constexpr int kScoreExp = 20;    // scores are kept in units of 2^kScoreExp, so that fp32 holds the factor of every K exponent
+constexpr float kScoreUnit = 1 << kScoreExp;
 constexpr int kWeightExp = 120;  // weights enter the product as p * 2^(e - R + kWeightExp)
 
 // kN: eights of query rows
@@ -238,7 +239,7 @@ attn_few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
     // this lane's key: its exponents as factors of a score and of a weight, and R
     const int left = key1 - first;
     const int ref_new = max(ref_v, __reduce_max_sync(0xffffffffu, exp_v));
-    float fk = fmaxf(attnx::exp2_int(min(exp_k, kMaxScaleExp) + 133 - kQueryExp) * p.scale_log2, 1.17549435e-38f);
+    float fk = fmaxf(attnx::exp2_int(exp_k + 133 - kQueryExp - kScoreExp) * p.scale_log2, 1.17549435e-38f);
     float fv = attnx::exp2_int(exp_v - ref_new + kWeightExp);
     if (exp_k == q8::kNotFinite) fk = NAN;
     if (exp_v == q8::kNotFinite) fv = NAN;
@@ -262,20 +263,6 @@ attn_few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
 #pragma unroll
           for (int i = 0; i < 4; ++i) s[kb][nb][i] *= row_fix[nb][i & 1];
     }
-    if (__any_sync(0xffffffffu, exp_k > kMaxScaleExp)) {  // what fk could not take
-      const float rest = attnx::exp2_int(max(exp_k - kMaxScaleExp, 0));
-#pragma unroll
-      for (int kb = 0; kb < kBlocks; ++kb)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const float f = __shfl_sync(0xffffffffu, rest, kb * 16 + i * 8 + g);
-#pragma unroll
-          for (int nb = 0; nb < kN; ++nb) {
-            s[kb][nb][2 * i] *= f;
-            s[kb][nb][2 * i + 1] *= f;
-          }
-        }
-    }
     if (left < kKeys) {
 #pragma unroll
       for (int kb = 0; kb < kBlocks; ++kb)
@@ -297,6 +284,7 @@ attn_few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
         for (int kb = 1; kb < kBlocks; ++kb) x = fmaxf(x, fmaxf(s[kb][nb][i], s[kb][nb][2 + i]));
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+        x *= kScoreUnit;
         mx[nb][i] = x;
         grow = grow || x > m[nb][i];
       }
@@ -329,7 +317,7 @@ attn_few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
           float w[2];
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
-            w[q] = ex2_approx(s[kb][nb][2 * i + q] - (m[nb][q] == -INFINITY ? 0.f : m[nb][q]));
+            w[q] = ex2_approx(fmaf(s[kb][nb][2 * i + q], kScoreUnit, m[nb][q] == -INFINITY ? 0.f : -m[nb][q]));
             l[nb][q] += w[q];
           }
           // bf16 as in the tensor-core kernels: 2^-9 of the output, as much as its own rounding

@@ -358,8 +358,8 @@ def attn_kvcache_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
                     v_exp: torch.Tensor, seq_lens: Sequence[int], *, out: Optional[torch.Tensor] = None,
                     softmax_scale: Optional[float] = None) -> torch.Tensor:
     """`attn_kvcache` over an 8-bit cache: softmax(q k^T scale) v over the values that cache[b, :seq_lens[b]] holds
-    (bf16 q and output).  seq_lens[b] may be 0: that row's output is 0.  Cache rows may be broadcast.  Scores have to stay
-    within fp32's range.  Scratch comes from PyTorch's allocator; above 768 queries it holds bf16 K and V of a group of
+    (bf16 q and output).  seq_lens[b] may be 0: that row's output is 0.  Cache rows may be broadcast.  Scores, and
+    the scale times the largest K, have to stay within fp32's range.  Scratch comes from PyTorch's allocator; above 768 queries it holds bf16 K and V of a group of
     heads, about 1 GiB at most (one head at least).  No gradient is recorded."""
     args = (q, k_cache, v_cache, k_exp, v_exp, seq_lens, out, softmax_scale, _status_ptr(q))
     if _log is None:
